@@ -38,6 +38,18 @@ class _Hparams(ctypes.Structure):
     ]
 
 
+class _AttnParams(ctypes.Structure):
+    _fields_ = (
+        [(n, ctypes.c_int) for n in ("dtype", "n_head", "n_head_kv", "head_dim", "n_seqs", "q_rows", "k_rows", "max_q",
+                                     "max_k")]
+        + [(n, ctypes.c_int64) for n in ("q_row_stride", "q_head_stride", "k_row_stride", "k_head_stride",
+                                         "v_row_stride", "v_head_stride", "out_row_stride", "out_head_stride")]
+        + [("d_cu_q", ctypes.c_void_p), ("d_cu_k", ctypes.c_void_p), ("scale", ctypes.c_float),
+           ("softcap", ctypes.c_float), ("window_left", ctypes.c_int), ("window_right", ctypes.c_int)]
+        + [(n, ctypes.c_void_p) for n in ("d_prefix", "d_doc_q", "d_doc_k", "d_slopes", "d_rel_bias")]
+        + [("rel_bias_radius", ctypes.c_int)])
+
+
 def load_library(path: Optional[str] = None):
     """Load (never build) the shared library; raises if it is missing."""
     global _lib
@@ -103,7 +115,16 @@ def load_library(path: Optional[str] = None):
                         ctypes.c_int, vp, vp], ctypes.c_int),
         "ceb_linear_create": ([ctypes.c_int, vp, ctypes.c_int, ctypes.c_int], vp),
         "ceb_linear_forward": ([vp, vp, ctypes.c_int, vp, ctypes.c_int, ctypes.c_int, vp, vp], ctypes.c_int),
+        "ceb_linear_fused": ([vp, vp, ctypes.c_int64, ctypes.c_int, vp, ctypes.c_int, vp, ctypes.c_int, ctypes.c_int64,
+                              ctypes.c_int, vp, ctypes.c_int64, vp], ctypes.c_int),
         "ceb_linear_free": ([vp], None),
+        "ceb_attention_masked": ([ctypes.POINTER(_AttnParams), vp, vp, vp, vp, vp], ctypes.c_int),
+        "ceb_rope_create": ([ctypes.c_int, ctypes.c_double, ctypes.c_int, ctypes.c_double, ctypes.c_int,
+                             ctypes.c_double, ctypes.c_double], vp),
+        "ceb_rope_forward": ([vp, vp, vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64,
+                              ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, vp, vp, ctypes.c_int,
+                              ctypes.c_int, vp], ctypes.c_int),
+        "ceb_rope_free": ([vp], None),
         "ceb_launch_count": ([], ctypes.c_longlong),
         "ceb_profile_enable": ([ctypes.c_int], None),
         "ceb_profile_read": ([ctypes.POINTER(ctypes.c_longlong), ctypes.POINTER(ctypes.c_double),
@@ -139,6 +160,30 @@ def _stream_ptr(stream) -> Optional[int]:
 
 def _ptr(t) -> Optional[int]:
     return None if t is None else t.data_ptr()
+
+
+def _need(ok: bool, what: str):
+    if not ok:
+        raise CrispEmbedError(what)
+
+
+def _on(x, what: str, **tensors):
+    """The device of `x` (a CUDA tensor); every other tensor given must lie there too."""
+    _need(x.is_cuda, f"{what}: CUDA tensors expected")
+    for name, t in tensors.items():
+        _need(t is None or t.device == x.device, f"{what}: {name} is on {getattr(t, 'device', None)}, not {x.device}")
+    return x.device
+
+
+def _vector(t, dtype, n: int, what: str):
+    """`t` (None allowed) is a contiguous vector of n values of `dtype`."""
+    _need(t is None or (t.dtype == dtype and t.numel() == n and t.is_contiguous()),
+          f"{what}: {n} contiguous values of {dtype} expected")
+
+
+def _act_types():
+    import torch
+    return {torch.float32: ACT_F32, torch.bfloat16: ACT_BF16, torch.float16: ACT_F16}
 
 
 class CrispEmbed:
@@ -392,6 +437,9 @@ class ExpertParallel:
             pass
 
 
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
 class Linear:
     """Device-resident linear layer (ceb_linear_create / ceb_linear_forward)."""
 
@@ -410,6 +458,32 @@ class Linear:
                               device=x.device)
         _check(self._lib.ceb_linear_forward(self._h, x.data_ptr(), x.shape[0], _ptr(bias), int(gelu), int(out_f16),
                                             out.data_ptr(), _stream_ptr(stream)), "ceb_linear_forward")
+        return out
+
+    def fused(self, x, bias=None, act: str = "none", residual=None, out=None, out_dtype=None, stream=None):
+        """act(x W^T + bias) + residual (ceb_linear_fused), rounded once to the output's type.
+
+        x: [m, k] fp16; residual, out: [m, n_out] in fp32, fp16 or bf16; rows may be strided.
+        act: "none", "relu", "silu", "gelu" or "gelu_tanh".  out (default: new, of out_dtype or
+        fp16) may be the residual.  Runs on x's device and its current stream."""
+        import torch
+        types = _act_types()
+        _need(act in ACTIVATIONS, f"fused: activation {act!r}: one of {', '.join(ACTIVATIONS)}")
+        _need(x.dim() == 2 and x.shape[1] == self.k and x.dtype == torch.float16 and x.stride(1) == 1,
+              f"fused: x must be fp16 [rows, {self.k}] with contiguous rows")
+        dev = _on(x, "fused", bias=bias, residual=residual, out=out)
+        _vector(bias, torch.float32, self.n_out, "fused: bias")
+        if out is None:
+            out = torch.empty((x.shape[0], self.n_out), dtype=out_dtype or torch.float16, device=dev)
+        for name, t in (("residual", residual), ("out", out)):
+            _need(t is None or (t.dtype in types and t.shape == (x.shape[0], self.n_out) and t.stride(1) == 1),
+                  f"fused: {name} must be [{x.shape[0]}, {self.n_out}] in fp32, fp16 or bf16 with contiguous rows")
+        _need(out_dtype is None or out.dtype == out_dtype, "fused: out is not of out_dtype")
+        with torch.cuda.device(dev):
+            _check(self._lib.ceb_linear_fused(
+                self._h, x.data_ptr(), x.stride(0), x.shape[0], _ptr(bias), ACTIVATIONS[act], _ptr(residual),
+                0 if residual is None else types[residual.dtype], 0 if residual is None else residual.stride(0),
+                types[out.dtype], out.data_ptr(), out.stride(0), _stream_ptr(stream)), "ceb_linear_fused")
         return out
 
     def close(self):
@@ -460,6 +534,117 @@ def attention(qkv, cu_seqlens, n_head: int, max_len: Optional[int] = None, strea
     _check(lib.ceb_attention_forward(qkv.data_ptr(), rows, cu_seqlens.data_ptr(), n, max_len, d, n_head,
                                      out.data_ptr(), _stream_ptr(stream)), "ceb_attention_forward")
     return out
+
+
+def attention_masked(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, max_k: Optional[int] = None, *,
+                     scale: Optional[float] = None, softcap: float = 0.0, window=(-1, -1), prefix=None, doc_q=None,
+                     doc_k=None, slopes=None, rel_bias=None, out=None, stream=None):
+    """Packed attention with shared key heads, a capped score, a bias by distance and masks
+    (ceb_attention_masked, whose header has the formulas).
+
+    q: [q_rows, n_head, head_dim], k / v: [k_rows, n_head_kv, head_dim], fp16 or bf16, any row and
+    head strides that are multiples of 8 values; cu_q / cu_k (default: cu_q) int32 row offsets;
+    max_q / max_k: the longest sequence (default: read from the offsets, which waits for the
+    device).  scale: default 1/sqrt(head_dim).  window: (left, right) keys around a row's place,
+    -1 open; (-1, 0) is causal.  prefix: int32 [n_seqs] keys that every row sees.  doc_q / doc_k:
+    int32 document numbers (doc_k default: doc_q).  slopes: fp32 [n_head], or rel_bias: fp32
+    [n_head, 2 R + 1].  Returns out, [q_rows, n_head, head_dim]; rows of no sequence are not
+    written.  Runs on q's device and its current stream."""
+    import torch
+    types = {t: c for t, c in _act_types().items() if t != torch.float32}
+    _need(q.dtype in types and k.dtype == q.dtype and v.dtype == q.dtype, "attention_masked: q, k, v in fp16 or bf16")
+    _need(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape and k.shape[2] == q.shape[2],
+          "attention_masked: q [rows, heads, head_dim], k and v [keys, key heads, head_dim] expected")
+    _need(all(t.stride(2) == 1 for t in (q, k, v)), "attention_masked: the values of a head must be contiguous")
+    cu_k = cu_q if cu_k is None else cu_k
+    doc_k = doc_q if doc_k is None else doc_k
+    dev = _on(q, "attention_masked", k=k, v=v, cu_q=cu_q, cu_k=cu_k, prefix=prefix, doc_q=doc_q, doc_k=doc_k,
+              slopes=slopes, rel_bias=rel_bias, out=out)
+    rows, n_head, hd = q.shape
+    n = cu_q.numel() - 1
+    _need(n >= 0, "attention_masked: row offsets expected")
+    _vector(cu_q, torch.int32, n + 1, "attention_masked: cu_q")
+    _vector(cu_k, torch.int32, n + 1, "attention_masked: cu_k")
+    _vector(prefix, torch.int32, n, "attention_masked: prefix")
+    _vector(doc_q, torch.int32, rows, "attention_masked: doc_q")
+    _vector(doc_k, torch.int32, k.shape[0], "attention_masked: doc_k")
+    _vector(slopes, torch.float32, n_head, "attention_masked: slopes")
+    radius = 0
+    if rel_bias is not None:
+        _need(rel_bias.dim() == 2 and rel_bias.shape[1] % 2 == 1, "attention_masked: rel_bias [heads, 2 R + 1] expected")
+        radius = rel_bias.shape[1] // 2
+        _vector(rel_bias, torch.float32, n_head * (2 * radius + 1), "attention_masked: rel_bias")
+    left, right = window
+    longest = [int((c[1:] - c[:-1]).max().item()) if given is None and n else given or 0
+               for c, given in ((cu_q, max_q), (cu_k, max_k))]
+    if out is None:
+        out = torch.empty((rows, n_head, hd), dtype=q.dtype, device=dev)
+    _need(out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1,
+          "attention_masked: out must have q's shape and type, the values of a head contiguous")
+    p = _AttnParams(types[q.dtype], n_head, k.shape[1], hd, n, rows, k.shape[0], longest[0], longest[1],
+                    q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0),
+                    out.stride(1), _ptr(cu_q), _ptr(cu_k), hd ** -0.5 if scale is None else scale, softcap, left, right,
+                    _ptr(prefix), _ptr(doc_q), _ptr(doc_k), _ptr(slopes), _ptr(rel_bias), radius)
+    with torch.cuda.device(dev):
+        _check(load_library().ceb_attention_masked(ctypes.byref(p), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                                   out.data_ptr(), _stream_ptr(stream)), "ceb_attention_masked")
+    return out
+
+
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+
+class Rope:
+    """Rotary positions: a plan of frequencies (ceb_rope_create) and the rotation (ceb_rope_forward)."""
+
+    def __init__(self, rot_dim: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                 context: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0):
+        """The plan lies on the current device.  scaling: "none", "linear", "ntk" or "yarn"."""
+        _need(scaling in ROPE_SCALINGS, f"Rope: scaling {scaling!r}: one of {', '.join(ROPE_SCALINGS)}")
+        self._h = None
+        self._lib = load_library()
+        self.rot_dim = rot_dim
+        self._h = self._lib.ceb_rope_create(rot_dim, theta, ROPE_SCALINGS[scaling], factor, context, beta_fast,
+                                            beta_slow)
+        if not self._h:
+            raise CrispEmbedError(f"ceb_rope_create failed: {last_error()}")
+
+    def __call__(self, x, out=None, positions=None, cu_seqlens=None, pos_offset: int = 0, interleaved: bool = False,
+                 stream=None):
+        """x: [rows, heads, head_dim] in fp32, fp16 or bf16, rows and heads strided at will.  Positions:
+        int32 [rows], or the rows' places in the sequences of cu_seqlens (int32) plus pos_offset.
+        out (default: new) may be x.  Runs on x's device and its current stream."""
+        import torch
+        types = _act_types()
+        _need(x.dim() == 3 and x.dtype in types and (x.stride(2) == 1 or x.shape[2] == 1),
+              "Rope: x must be [rows, heads, head_dim] in fp32, fp16 or bf16, the values of a head contiguous")
+        dev = _on(x, "Rope", out=out, positions=positions, cu_seqlens=cu_seqlens)
+        _need(positions is not None or cu_seqlens is not None, "Rope: positions or cu_seqlens must be given")
+        _vector(positions, torch.int32, x.shape[0], "Rope: positions")
+        if cu_seqlens is not None:
+            _vector(cu_seqlens, torch.int32, cu_seqlens.numel(), "Rope: cu_seqlens")
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        _need(out.shape == x.shape and out.dtype == x.dtype and out.stride(2) == 1,
+              "Rope: out must have x's shape and type, the values of a head contiguous")
+        n = 0 if cu_seqlens is None else cu_seqlens.numel() - 1
+        with torch.cuda.device(dev):
+            _check(self._lib.ceb_rope_forward(self._h, x.data_ptr(), out.data_ptr(), types[x.dtype], x.shape[0],
+                                              x.shape[1], x.shape[2], x.stride(0), x.stride(1), out.stride(0),
+                                              out.stride(1), int(interleaved), _ptr(positions), _ptr(cu_seqlens), n,
+                                              pos_offset, _stream_ptr(stream)), "ceb_rope_forward")
+        return out
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self._lib.ceb_rope_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def gguf_dequantize(ggml_type: int, raw: np.ndarray, n_rows: int, k: int) -> np.ndarray:

@@ -710,19 +710,31 @@ namespace {
 constexpr int OP_MAX_DEVICES = 64;
 int* g_op_err[OP_MAX_DEVICES] = {};
 std::mutex g_op_mu;
+// A zeroed device allocation that may be made while the caller's stream is captured: the
+// calling thread leaves the capture's rules for the moment, and the clearing runs on a
+// stream of its own, so that neither becomes part of the graph nor ends the capture.
+int* zeroed_words(int n) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+    int* p = nullptr;
+    cudaStream_t own = nullptr;
+    bool ok = cudaMalloc(&p, n * sizeof(int)) == cudaSuccess;
+    ok = ok && cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking) == cudaSuccess;
+    ok = ok && cudaMemsetAsync(p, 0, n * sizeof(int), own) == cudaSuccess;
+    ok = ok && cudaStreamSynchronize(own) == cudaSuccess;
+    if (own) cudaStreamDestroy(own);
+    if (!ok && p) {
+        cudaFree(p);
+        p = nullptr;
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return ok ? p : nullptr;
+}
 int* op_err_word() {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= OP_MAX_DEVICES) return nullptr;
     std::lock_guard<std::mutex> lk(g_op_mu);
-    if (!g_op_err[dev]) {
-        int* p = nullptr;
-        if (cudaMalloc(&p, sizeof(int)) != cudaSuccess) return nullptr;
-        if (cudaMemset(p, 0, sizeof(int)) != cudaSuccess) {
-            cudaFree(p);
-            return nullptr;
-        }
-        g_op_err[dev] = p;
-    }
+    if (!g_op_err[dev]) g_op_err[dev] = zeroed_words(1);
     return g_op_err[dev];
 }
 }  // namespace
@@ -856,6 +868,7 @@ extern "C" int ceb_attention_forward(const void* d_qkv, int n_rows, const int32_
 
 struct ceb_linear {
     ceb_wplane w;
+    int device = 0;
 };
 
 extern "C" ceb_linear* ceb_linear_create(int w_type, const void* h_w, int n_out, int k) {
@@ -868,6 +881,7 @@ extern "C" ceb_linear* ceb_linear_create(int w_type, const void* h_w, int n_out,
         delete L;
         return nullptr;
     }
+    cudaGetDevice(&L->device);
     return L;
 }
 
@@ -884,6 +898,73 @@ extern "C" int ceb_linear_forward(const ceb_linear* L, const void* d_x, int m, c
     a.epi = (out_f16 ? CEB_EPI_F16_OUT : 0) | (gelu ? CEB_EPI_GELU : 0) | (d_bias ? CEB_EPI_BIAS : 0);
     a.bias = d_bias;
     a.err = err;
+    return ceb_gemm_launch(L->w, d_x, m, a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ceb_linear_fused(const ceb_linear* L, const void* d_x, int64_t x_stride, int m, const float* d_bias,
+                                int act, const void* d_residual, int residual_dtype, int64_t residual_stride,
+                                int out_dtype, void* d_out, int64_t out_stride, void* stream) {
+    if (!L || m < 0) return ceb_set_error(1, "linear_fused: bad arguments");
+    auto size_of = [](int dtype) {
+        return dtype == CEB_ACT_F32 ? 4 : dtype == CEB_ACT_F16 || dtype == CEB_ACT_BF16 ? 2 : 0;
+    };
+    if (act < CEB_FN_NONE || act > CEB_FN_GELU_TANH) return ceb_set_error(1, "linear_fused: unknown activation %d", act);
+    const int osz = size_of(out_dtype), rsz = d_residual ? size_of(residual_dtype) : 4;
+    if (!osz || !rsz) return ceb_set_error(1, "linear_fused: unknown output or residual type");
+    if (m == 0) return 0;
+    if (!d_x || !d_out) return ceb_set_error(1, "linear_fused: null tensor");
+    const int n = L->w.n_out, k = L->w.k;
+    if (m == 1) {  // one row has no stride
+        x_stride = k;
+        out_stride = residual_stride = n;
+    }
+    constexpr int64_t FAR = (int64_t)1 << 38;  // a tensor map's strides end at 2^40 bytes
+    if (x_stride < k || x_stride > FAR || x_stride % 8 || out_stride < n || out_stride > FAR ||
+        out_stride * osz % 16 || (d_residual && (residual_stride < n || residual_stride > FAR ||
+                                                 residual_stride * rsz % 16)))
+        return ceb_set_error(1, "linear_fused: row strides must hold a row and be multiples of 16 bytes");
+    if ((reinterpret_cast<uintptr_t>(d_x) | reinterpret_cast<uintptr_t>(d_out) |
+         reinterpret_cast<uintptr_t>(d_residual)) & 15)
+        return ceb_set_error(1, "linear_fused: x, residual and out must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(d_bias) & 3) return ceb_set_error(1, "linear_fused: bias not aligned");
+    const uint8_t* o = static_cast<const uint8_t*>(d_out);
+    auto span = [&](int64_t stride, int cols, int size) {  // in doubles' range: no tensor is this large
+        return (uint64_t)std::min(((double)(m - 1) * stride + cols) * size, 9e15);
+    };
+    const uint64_t span_o = span(out_stride, n, osz);
+    auto overlaps = [&](const void* x, uint64_t bytes) {
+        const uint8_t* b = static_cast<const uint8_t*>(x);
+        return b < o + span_o && o < b + bytes;
+    };
+    const bool in_place = d_residual == d_out && residual_dtype == out_dtype && residual_stride == out_stride;
+    if (overlaps(d_x, span(x_stride, k, 2)) ||
+        (d_residual && !in_place && overlaps(d_residual, span(residual_stride, n, rsz))))
+        return ceb_set_error(1, "linear_fused: out overlaps an input");
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) return ceb_set_error(3, "linear_fused: no current device");
+    if (dev != L->device)
+        return ceb_set_error(1, "linear_fused: layer of device %d used on device %d", L->device, dev);
+    int* err = op_err_word();
+    if (!err) return ceb_set_error(4, "out of device memory");
+    ceb_gemm_args a;
+    a.m_rows = m;
+    a.out = d_out;
+    a.ldo = out_stride;
+    a.epi = d_bias ? CEB_EPI_BIAS : 0;
+    a.bias = d_bias;
+    a.err = err;
+    a.ldx = x_stride;
+    if (!d_residual && out_dtype != CEB_ACT_BF16 && (act == CEB_FN_NONE || act == CEB_FN_GELU)) {
+        // what ceb_linear_forward computes
+        a.epi |= (out_dtype == CEB_ACT_F16 ? CEB_EPI_F16_OUT : 0) | (act == CEB_FN_GELU ? CEB_EPI_GELU : 0);
+    } else {
+        a.ex = true;
+        a.act = act;
+        a.out_type = out_dtype;
+        a.res = d_residual;
+        a.res_type = residual_dtype;
+        a.ldr = residual_stride;
+    }
     return ceb_gemm_launch(L->w, d_x, m, a, static_cast<cudaStream_t>(stream));
 }
 

@@ -76,12 +76,20 @@ struct ceb_gemm_args {
     const int* offsets = nullptr;  // device [n_groups+1] activation-row ranges per group; null = dense
     int m_rows = 0;                // dense: activation rows; grouped: capacity of the activation buffer
     void* out = nullptr;
-    int ldo = 0;                   // output row stride (elements)
+    int64_t ldo = 0;               // output row stride (elements)
     int epi = 0;
     const float* bias = nullptr;
     int64_t bias_group_stride = 0;
     int* err = nullptr;            // device error word
     int prof_cat = CEB_PROF_GEMM;  // profiling category of the launch
+    // the extended epilogue (ceb_linear_fused): act(acc + bias) + residual, rounded once
+    bool ex = false;               // run it; epi then holds CEB_EPI_BIAS at most, and the output type is out_type
+    int act = 0;                   // CEB_FN_*
+    int out_type = 0;              // CEB_ACT_*
+    const void* res = nullptr;     // residual rows (null: none), may be `out`
+    int res_type = 0;              // CEB_ACT_*
+    int64_t ldr = 0;               // residual row stride (elements)
+    int64_t ldx = 0;               // activation row stride (elements; 0: k)
 };
 
 // status / errors

@@ -40,6 +40,7 @@
 #include <cstdio>
 #include <cstdlib>
 
+#include "../../include/ceb_ops.h"
 #include "ceb_internal.h"
 #include "common.cuh"
 
@@ -285,7 +286,41 @@ CEB_DEV f32x2 gelu_as2(f32x2 x) {
     return f2_fma(f2_mul(ax, f2_splat(0.5f)), erf_abs, h);
 }
 
-template <int FMT>
+// Activations of the extended epilogue.  silu(x) = x / (1 + exp(-x)); the tanh form of GELU
+// is the same with 2 sqrt(2/pi) (x + 0.044715 x^3) in the exponent, since
+// (1 + tanh u) / 2 = 1 / (1 + exp(-2u)).  Exponential and reciprocal are the MUFU
+// approximations (relative error ~2^-22, below the fp32 sums in front of them).
+CEB_DEV float ex_act(float x, int act) {
+    if (act == CEB_FN_GELU) return gelu_as(x);
+    if (act == CEB_FN_RELU) return x < 0.0f ? 0.0f : x;  // NaN stays
+    if (act == CEB_FN_NONE) return x;
+    constexpr float kL = 1.4426950408889634f, kG = 2.0f * 0.79788456080286536f;
+    const float u = act == CEB_FN_SILU ? x : kG * fmaf(0.044715f * x * x, x, x);
+    return x * rcp_approx(1.0f + ex2_approx(-kL * u));
+}
+// four consecutive values of type CEB_ACT_* at element `i` of `p` (aligned to four values)
+CEB_DEV float4 load4(const void* p, int type, int64_t i) {
+    if (type == CEB_ACT_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+    if (type == CEB_ACT_BF16)
+        return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                           __uint_as_float(u.y & 0xffff0000u));
+    const float2 a = __half22float2(u32_as_h2(u.x)), b = __half22float2(u32_as_h2(u.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+CEB_DEV float load1(const void* p, int type, int64_t i) {
+    if (type == CEB_ACT_F32) return static_cast<const float*>(p)[i];
+    if (type == CEB_ACT_F16) return __half2float(static_cast<const __half*>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+// two values as the packed 16-bit pair of type `type`
+CEB_DEV uint32_t pack2(float a, float b, int type) {
+    if (type == CEB_ACT_F16) return h2_as_u32(__floats2half2_rn(a, b));
+    __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&r);
+}
+
+template <int FMT, bool EX>
 __global__ void __launch_bounds__(NTHREADS, 1)
     ceb_gemm_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap omap,
                     const ceb_wplane w, const ceb_gemm_args a) {
@@ -468,8 +503,14 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         const int wg = ew >> 2;                  // this warpgroup takes 32-column chunks c with c % EPI_WG == wg
         const int q = warp & 3;                  // features 32q .. 32q+31 of the tile (TMEM lanes)
         const uint32_t lane_addr = (uint32_t)(32 * q) << 16;
-        const bool f16 = (a.epi & CEB_EPI_F16_OUT) != 0, gelu = (a.epi & CEB_EPI_GELU) != 0;
+        const bool f16 = EX ? a.out_type != CEB_ACT_F32 : (a.epi & CEB_EPI_F16_OUT) != 0;
+        const bool gelu = (a.epi & CEB_EPI_GELU) != 0;
         const int esz = f16 ? 2 : 4;
+        // one value in the 16-bit output type
+        auto out16 = [&](float v) {
+            return EX && a.out_type == CEB_ACT_BF16 ? __ushort_as_half(__bfloat16_as_ushort(__float2bfloat16_rn(v)))
+                                                    : __float2half_rn(v);
+        };
         uint8_t* slot = SH.staging + (size_t)ew * STAGING_SLOT;
         uint32_t lt = 0, nstore = 0;
         for (int t = blockIdx.x; t < total; t += gridDim.x, ++lt) {
@@ -490,9 +531,15 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
                     x[j] = __uint_as_float(v[j]) + bv;
-                    if (gelu) x[j] = gelu_as(x[j]);
+                    if (EX) x[j] = ex_act(x[j], a.act);
+                    else if (gelu) x[j] = gelu_as(x[j]);
                 }
                 const int lim = ti.rows - c0;
+                if (EX && a.res) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (j < lim) x[j] += load1(a.res, a.res_type, (int64_t)(ti.row0 + c0 + j) * a.ldr + n);
+                }
                 if (CEB_GEMM_TMA_STORE && lim >= 32) {
                     // full 32-row block: stage [row][feature] in shared memory, one TMA store
                     if (nstore >= 1) {  // the previous store has finished reading the slot
@@ -502,7 +549,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     if (f16) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
-                            reinterpret_cast<__half*>(slot)[j * 32 + lane] = __float2half_rn(x[j]);
+                            reinterpret_cast<__half*>(slot)[j * 32 + lane] = out16(x[j]);
                     } else {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) reinterpret_cast<float*>(slot)[j * 32 + lane] = x[j];
@@ -518,7 +565,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     __half* o = reinterpret_cast<__half*>(a.out) + (size_t)(ti.row0 + c0) * a.ldo + n;
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
-                        if (j < lim) o[(size_t)j * a.ldo] = __float2half_rn(x[j]);
+                        if (j < lim) o[(size_t)j * a.ldo] = out16(x[j]);
                 } else {
                     float* o = reinterpret_cast<float*>(a.out) + (size_t)(ti.row0 + c0) * a.ldo + n;
 #pragma unroll
@@ -542,11 +589,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     }
 }
 
-template <int FMT>
+template <int FMT, bool EX>
 int launch_fmt(const CUtensorMap& map, const CUtensorMap& omap, const ceb_wplane& w, const ceb_gemm_args& a, int grid,
                cudaStream_t st) {
-    if (int rc = ceb_func_smem(reinterpret_cast<const void*>(ceb_gemm_kernel<FMT>), SMEM_BYTES)) return rc;
-    ceb_gemm_kernel<FMT><<<grid, NTHREADS, SMEM_BYTES, st>>>(map, omap, w, a);
+    if (int rc = ceb_func_smem(reinterpret_cast<const void*>(ceb_gemm_kernel<FMT, EX>), SMEM_BYTES)) return rc;
+    ceb_gemm_kernel<FMT, EX><<<grid, NTHREADS, SMEM_BYTES, st>>>(map, omap, w, a);
     CEB_CUDA_OK(cudaGetLastError());
     return 0;
 }
@@ -733,7 +780,7 @@ struct PairWarps {
     static constexpr int THREADS = 32 * (EPI0 + 4 * EPI_WG);
 };
 
-template <int FMT>
+template <int FMT, bool EX>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<FMT>::THREADS, 1)
     ceb_gemm_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap omap,
                          const __grid_constant__ CUtensorMap wmap, const ceb_wplane w, const ceb_gemm_args a) {
@@ -990,7 +1037,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<FMT>::THRE
         const int wg = ew >> 2;                 // columns (features) 128*wg .. 128*wg+127 of the pair tile
         const int q = warp & 3;                 // TMEM lanes (tokens) 32q .. 32q+31
         const uint32_t lane_addr = (uint32_t)(32 * q) << 16;
-        const bool f16 = (a.epi & CEB_EPI_F16_OUT) != 0, gelu = (a.epi & CEB_EPI_GELU) != 0;
+        const bool f16 = EX ? a.out_type != CEB_ACT_F32 : (a.epi & CEB_EPI_F16_OUT) != 0;
+        const bool gelu = !EX && (a.epi & CEB_EPI_GELU) != 0;
         constexpr int NSLOT = L::NSLOT;
         uint32_t lt = 0, nstore = 0;
         for (int t = pair_id; t < total; t += n_pairs, ++lt) {
@@ -1011,7 +1059,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<FMT>::THRE
                 // slots are used in turn; the store that last used this one has finished reading it
                 uint8_t* slot = SH.staging + (size_t)(ew * NSLOT + (int)(nstore % NSLOT)) * SLOT;
                 const uint32_t slot_u32 = smem_u32(slot);
-                if (kTmaW && gelu && f16) {
+                if (!EX && kTmaW && gelu && f16) {
                     // fc1 + GELU: the chunk's TMEM loads and GELU run before the wait for the store
                     // that last used this slot, so that store's read of shared memory hides behind
                     // the math (+4.5 % at M = 70,825). Without GELU the math is short and the
@@ -1053,11 +1101,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<FMT>::THRE
                         tmem_ld32(tmem + lane_addr + col0 + (uint32_t)(c0 + h), v);
                         tmem_ld_wait();
                         epi_math<kTmaW>(v, bias ? bias + f_base + c0 + h : nullptr, gelu);
-                        const float* x = reinterpret_cast<const float*>(v);
+                        float* x = reinterpret_cast<float*>(v);
+                        if constexpr (EX) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) x[j] = ex_act(x[j], a.act);
+                            if (a.res && lane < lim) {
+                                const int64_t at = (int64_t)(row + lane) * a.ldr + f_base + c0 + h;
+#pragma unroll
+                                for (int j = 0; j < 32; j += 4) {
+                                    const float4 r = load4(a.res, a.res_type, at + j);
+                                    x[j] += r.x;
+                                    x[j + 1] += r.y;
+                                    x[j + 2] += r.z;
+                                    x[j + 3] += r.w;
+                                }
+                            }
+                        }
                         if (f16) {
                             uint32_t p[16];
     #pragma unroll
-                            for (int j = 0; j < 16; ++j) p[j] = h2_as_u32(__floats2half2_rn(x[2 * j], x[2 * j + 1]));
+                            for (int j = 0; j < 16; ++j)
+                                p[j] = EX ? pack2(x[2 * j], x[2 * j + 1], a.out_type)
+                                          : h2_as_u32(__floats2half2_rn(x[2 * j], x[2 * j + 1]));
                             if (full) {  // 64 B = chunks 4*(h/32) .. +3 of the 128-B swizzled row
     #pragma unroll
                                 for (int c = 0; c < 4; ++c) {
@@ -1119,25 +1184,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<FMT>::THRE
     }
 }
 
-template <int FMT>
+template <int FMT, bool EX>
 int launch_pair(const CUtensorMap& xmap, const CUtensorMap& omap, const CUtensorMap& wmap, const ceb_wplane& w,
                 const ceb_gemm_args& a, int max_pairs, cudaStream_t st) {
     static int resident_of[CEB_MAX_DEVICES] = {};  // co-resident pairs, per device
     int& pairs_resident = resident_of[ceb_device_index()];
     if (!pairs_resident) {
-        if (int rc = ceb_func_smem(reinterpret_cast<const void*>(ceb_gemm_pair_kernel<FMT>), pair::LayOf<FMT>::SMEM))
+        if (int rc = ceb_func_smem(reinterpret_cast<const void*>(ceb_gemm_pair_kernel<FMT, EX>), pair::LayOf<FMT>::SMEM))
             return rc;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2 * ceb_num_sms(), 1, 1);
         cfg.blockDim = dim3(PairWarps<FMT>::THREADS, 1, 1);
         cfg.dynamicSmemBytes = pair::LayOf<FMT>::SMEM;
         int n = 0;  // cluster size comes from the kernel's __cluster_dims__
-        CEB_CUDA_OK(cudaOccupancyMaxActiveClusters(&n, ceb_gemm_pair_kernel<FMT>, &cfg));
+        CEB_CUDA_OK(cudaOccupancyMaxActiveClusters(&n, ceb_gemm_pair_kernel<FMT, EX>, &cfg));
         pairs_resident = n > 0 ? n : 1;
     }
     int pairs = pairs_resident < max_pairs ? pairs_resident : max_pairs;
     if (pairs < 1) pairs = 1;
-    ceb_gemm_pair_kernel<FMT><<<2 * pairs, PairWarps<FMT>::THREADS, pair::LayOf<FMT>::SMEM, st>>>(xmap, omap, wmap, w,
+    ceb_gemm_pair_kernel<FMT, EX><<<2 * pairs, PairWarps<FMT>::THREADS, pair::LayOf<FMT>::SMEM, st>>>(xmap, omap, wmap, w,
                                                                                                 a);
     CEB_CUDA_OK(cudaGetLastError());
     return 0;
@@ -1218,20 +1283,22 @@ int ceb_gemm_launch(const ceb_wplane& w, const void* act_f16, int act_rows, cons
     if (a.offsets && (w.n_groups < 1 || w.n_groups > MAXG))
         return ceb_set_error(2, "gemm: %d groups (max %d)", w.n_groups, MAXG);
     if ((reinterpret_cast<uintptr_t>(act_f16) & 15) != 0) return ceb_set_error(2, "gemm: activations not 16-B aligned");
-    if ((a.epi & CEB_EPI_F16_OUT) && (a.ldo & 1)) return ceb_set_error(2, "gemm: fp16 output stride must be even");
+    const bool out_f32 = a.ex ? a.out_type == CEB_ACT_F32 : !(a.epi & CEB_EPI_F16_OUT);
+    const int64_t ldx = a.ldx ? a.ldx : w.k;
+    if (!out_f32 && (a.ldo & 1)) return ceb_set_error(2, "gemm: fp16 output stride must be even");
     if (act_rows <= 0) return 0;
-    const int esz = (a.epi & CEB_EPI_F16_OUT) ? 2 : 4;
+    const int esz = out_f32 ? 4 : 2;
     if ((reinterpret_cast<uintptr_t>(a.out) & 15) || ((size_t)a.ldo * esz) % 16 || a.ldo < w.n_out)
         return ceb_set_error(2, "gemm: output must be 16-B aligned with a row stride >= n_out and a multiple of 16 B");
     const int groups = a.offsets ? w.n_groups : 1;
     const double flops = 2.0 * (double)a.m_rows * w.n_out * w.k;
     const double bytes = (double)(w.q_bytes + w.s_bytes) + (double)a.m_rows * w.k * 2 +
-                         (double)a.m_rows * w.n_out * ((a.epi & CEB_EPI_F16_OUT) ? 2 : 4);
+                         (double)a.m_rows * w.n_out * (esz + (!a.res ? 0 : a.res_type == CEB_ACT_F32 ? 4 : 2));
     CUtensorMap map, omap;
     int mrc = 0;
     if (ceb_gemm_use_pairs(w, a)) {
         // CTA-pair kernel: 128-token activation boxes, 128-byte-swizzled 32-row output boxes
-        mrc = ceb_make_tmap_2d_f16(&map, act_f16, (uint64_t)w.k, (uint64_t)act_rows, (uint64_t)w.k * 2, BK, pair::TOK);
+        mrc = ceb_make_tmap_2d_f16(&map, act_f16, (uint64_t)w.k, (uint64_t)act_rows, (uint64_t)ldx * 2, BK, pair::TOK);
         if (mrc) return mrc;
         mrc = ceb_make_tmap_2d(&omap, a.out, esz, (uint64_t)w.n_out, (uint64_t)a.m_rows, (uint64_t)a.ldo * esz,
                                esz == 2 ? 64 : 32, 32, true);
@@ -1249,14 +1316,14 @@ int ceb_gemm_launch(const ceb_wplane& w, const void* act_f16, int act_rows, cons
         }
         int rc = 0;
         switch (w.format) {
-            case CEB_W_Q8_0: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = launch_pair<CEB_W_Q8_0>(map, omap, wmap, w, a, max_pairs, stream)); break;
-            case CEB_W_Q4_K: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = launch_pair<CEB_W_Q4_K>(map, omap, wmap, w, a, max_pairs, stream)); break;
-            case CEB_W_F16: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = launch_pair<CEB_W_F16>(map, omap, wmap, w, a, max_pairs, stream)); break;
+            case CEB_W_Q8_0: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = a.ex ? launch_pair<CEB_W_Q8_0, true>(map, omap, wmap, w, a, max_pairs, stream) : launch_pair<CEB_W_Q8_0, false>(map, omap, wmap, w, a, max_pairs, stream)); break;
+            case CEB_W_Q4_K: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = a.ex ? launch_pair<CEB_W_Q4_K, true>(map, omap, wmap, w, a, max_pairs, stream) : launch_pair<CEB_W_Q4_K, false>(map, omap, wmap, w, a, max_pairs, stream)); break;
+            case CEB_W_F16: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = a.ex ? launch_pair<CEB_W_F16, true>(map, omap, wmap, w, a, max_pairs, stream) : launch_pair<CEB_W_F16, false>(map, omap, wmap, w, a, max_pairs, stream)); break;
             default: return ceb_set_error(2, "gemm: unknown weight format %d", w.format);
         }
         return rc;
     }
-    mrc = ceb_make_tmap_2d_f16(&map, act_f16, (uint64_t)w.k, (uint64_t)act_rows, (uint64_t)w.k * 2, BK, BN);
+    mrc = ceb_make_tmap_2d_f16(&map, act_f16, (uint64_t)w.k, (uint64_t)act_rows, (uint64_t)ldx * 2, BK, BN);
     if (mrc) return mrc;
     mrc = ceb_make_tmap_2d(&omap, a.out, esz, (uint64_t)w.n_out, (uint64_t)a.m_rows, (uint64_t)a.ldo * esz, 32, 32,
                            false);
@@ -1268,9 +1335,9 @@ int ceb_gemm_launch(const ceb_wplane& w, const void* act_f16, int act_rows, cons
     if (bound < grid) grid = (int)bound;
     int rc = 0;
     switch (w.format) {
-        case CEB_W_Q8_0: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = launch_fmt<CEB_W_Q8_0>(map, omap, w, a, grid, stream)); break;
-        case CEB_W_Q4_K: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = launch_fmt<CEB_W_Q4_K>(map, omap, w, a, grid, stream)); break;
-        case CEB_W_F16: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = launch_fmt<CEB_W_F16>(map, omap, w, a, grid, stream)); break;
+        case CEB_W_Q8_0: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = a.ex ? launch_fmt<CEB_W_Q8_0, true>(map, omap, w, a, grid, stream) : launch_fmt<CEB_W_Q8_0, false>(map, omap, w, a, grid, stream)); break;
+        case CEB_W_Q4_K: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = a.ex ? launch_fmt<CEB_W_Q4_K, true>(map, omap, w, a, grid, stream) : launch_fmt<CEB_W_Q4_K, false>(map, omap, w, a, grid, stream)); break;
+        case CEB_W_F16: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = a.ex ? launch_fmt<CEB_W_F16, true>(map, omap, w, a, grid, stream) : launch_fmt<CEB_W_F16, false>(map, omap, w, a, grid, stream)); break;
         default: return ceb_set_error(2, "gemm: unknown weight format %d", w.format);
     }
     return rc;

@@ -273,6 +273,93 @@ CEB_API int ceb_attention_forward(const void* d_qkv, int n_rows, const int32_t* 
                                   int d, int n_head, void* d_out, void* stream);
 
 /*
+ * Attention over packed sequences with shared key heads, score capping, a bias by
+ * distance and masks (no counterpart in the reference's MoE graph, whose attention is
+ * ceb_attention_forward's).  Sequence s has query rows cu_q[s] .. cu_q[s+1]-1 and key rows
+ * cu_k[s] .. cu_k[s+1]-1; query head h reads key head h / (n_head / n_head_kv).  Query
+ * row i of n takes the place i' = i + m - n among the sequence's m keys (its last row is
+ * level with the last key), and
+ *   t_ij  = scale * q_i . k_j
+ *   s_ij  = softcap * tanh(t_ij / softcap)        (softcap 0: s_ij = t_ij)
+ *   s_ij += -slopes[h] * |j - i'|                 (d_slopes given), or
+ *   s_ij += rel_bias[h][clamp(j - i', -R, R) + R] (d_rel_bias given, R = rel_bias_radius)
+ *   out_i = sum_j softmax_j(s_ij) v_j  over the keys row i may see,
+ * key j seen by row i if  (i' - window_left <= j <= i' + window_right  or  j < prefix[s])
+ * and doc_q[i] == doc_k[j].  A window side of -1 is open (window_right 0: causal); prefixes
+ * count keys; rows or keys of a negative document number see and are seen by nothing.  A
+ * row that sees no key, or only keys whose bias is -inf, gets zeros.  Keys that a row may
+ * not see have no part in its result, whatever they hold (inf and NaN included).
+ *
+ * q [q_rows x n_head x head_dim], k and v [k_rows x n_head_kv x head_dim], out as q, all of
+ * type dtype (CEB_ACT_F16 or CEB_ACT_BF16), 16-byte aligned, with strides in elements
+ * that are multiples of 8 (values of a head are contiguous).  head_dim: a multiple of 8 up
+ * to 128; n_head / n_head_kv <= 128.  max_q / max_k: at least the longest sequence of
+ * either side.  out may not overlap q, k or v; its rows that belong to no sequence stay as
+ * they were.  Scores, softmax statistics and sums are fp32; the softmax weights meet V in
+ * dtype.  No workspace, no state between calls: calls may overlap on any streams and may be
+ * captured.  Offsets that disagree with max_q / max_k or leave the rows set the device
+ * error word (status 5 of ceb_sync_check) and their sequence is skipped.
+ */
+typedef struct ceb_attn_params {
+    int dtype;
+    int n_head, n_head_kv, head_dim;
+    int n_seqs, q_rows, k_rows, max_q, max_k;
+    int64_t q_row_stride, q_head_stride;
+    int64_t k_row_stride, k_head_stride;
+    int64_t v_row_stride, v_head_stride;
+    int64_t out_row_stride, out_head_stride;
+    const int32_t* d_cu_q; /* [n_seqs + 1] */
+    const int32_t* d_cu_k; /* [n_seqs + 1] */
+    float scale;
+    float softcap;
+    int window_left, window_right;
+    const int32_t* d_prefix;  /* [n_seqs] or NULL */
+    const int32_t* d_doc_q;   /* [q_rows] or NULL (both or neither) */
+    const int32_t* d_doc_k;   /* [k_rows] */
+    const float* d_slopes;    /* [n_head] or NULL */
+    const float* d_rel_bias;  /* [n_head x (2 R + 1)] or NULL (not with slopes) */
+    int rel_bias_radius;
+} ceb_attn_params;
+CEB_API int ceb_attention_masked(const ceb_attn_params* p, const void* d_q, const void* d_k, const void* d_v,
+                                 void* d_out, void* stream);
+
+/*
+ * Rotary positions (the rotation in front of the attention of a model without a position
+ * table, src/crispembed.cpp:1182-1195, as an operator; scaled forms have no counterpart
+ * there).  A plan holds the rot_dim / 2 frequencies f_i = theta^(-2 i / rot_dim) on the
+ * current device in 64 bits, scaled for long contexts:
+ *   CEB_ROPE_LINEAR  f_i / factor
+ *   CEB_ROPE_NTK     theta * factor^(rot_dim / (rot_dim - 2)) in place of theta
+ *   CEB_ROPE_YARN    f_i / factor * g_i + f_i * (1 - g_i), g_i rising from 0 to 1 between the
+ *                    pairs that turn beta_fast and beta_slow times within `context` positions;
+ *                    cos and sin are stretched by 0.1 ln(factor) + 1
+ * factor >= 1; context, beta_fast and beta_slow are read by YARN only.  rot_dim: even, up to
+ * 256.  NULL on failure.
+ *
+ * ceb_rope_forward turns the first rot_dim values of every head of d_x [n_rows x n_head x
+ * head_dim] (strides in elements, values of a head contiguous) into d_out, pairing the
+ * values i and i + rot_dim/2 (interleaved 0) or 2i and 2i+1 (interleaved 1), and copies the
+ * values behind them.  Q and K heads that lie side by side in a row take one call.  The angle
+ * is position * f_i, reduced in 64 bits, the rotation fp32, rounded once to dtype (CEB_ACT_*).
+ * A row's position is d_positions[row] if given, else its distance from the start of its
+ * sequence (d_cu_seqlens [n_seqs + 1]) plus pos_offset; rows outside every sequence are left
+ * as they were.  d_out may be d_x (with the same strides), and may not overlap it otherwise.
+ * Asynchronous; no workspace.  The plan must be used on the device it was made on.
+ */
+#define CEB_ROPE_NONE 0
+#define CEB_ROPE_LINEAR 1
+#define CEB_ROPE_NTK 2
+#define CEB_ROPE_YARN 3
+typedef struct ceb_rope ceb_rope;
+CEB_API ceb_rope* ceb_rope_create(int rot_dim, double theta, int scaling, double factor, int context, double beta_fast,
+                                  double beta_slow);
+CEB_API int ceb_rope_forward(const ceb_rope* rope, const void* d_x, void* d_out, int dtype, int n_rows, int n_head,
+                             int head_dim, int64_t x_row_stride, int64_t x_head_stride, int64_t out_row_stride,
+                             int64_t out_head_stride, int interleaved, const int32_t* d_positions,
+                             const int32_t* d_cu_seqlens, int n_seqs, int pos_offset, void* stream);
+CEB_API void ceb_rope_free(ceb_rope* rope);
+
+/*
  * A device-resident linear layer (one ggml_mul_mat weight of the encoder,
  * src/crispembed.cpp:1160-1416): W [n_out rows x k] given as GGUF bytes on the
  * host, repacked once into the planes the tensor-core GEMM streams.
@@ -284,6 +371,25 @@ typedef struct ceb_linear ceb_linear;
 CEB_API ceb_linear* ceb_linear_create(int w_type, const void* h_w, int n_out, int k);
 CEB_API int ceb_linear_forward(const ceb_linear* lin, const void* d_x, int m, const float* d_bias, int gelu,
                                int out_f16, void* d_out, void* stream);
+/*
+ * The linear layer with its activation and the residual stream in the epilogue:
+ *   d_out[m, n] = act( sum_k W[n, k] * d_x[m, k] (+ d_bias[n]) ) (+ d_residual[m, n]),
+ * computed in fp32 and rounded once to out_dtype.  d_x [m x k] fp16 with rows x_stride
+ * elements apart (a multiple of 8, 16-byte aligned); d_residual (NULL: none) and d_out of
+ * type residual_dtype / out_dtype (CEB_ACT_*), 16-byte aligned, row strides a multiple of
+ * 16 bytes.  d_out may be d_residual itself (same type and
+ * stride), and may not overlap it or d_x otherwise.  act: CEB_FN_*.  Weights are rounded to
+ * fp16 where the stored blocks do not fit it, as in ceb_linear_forward.  Asynchronous; no
+ * workspace.  On the device that the layer was made on.
+ */
+#define CEB_FN_NONE 0
+#define CEB_FN_RELU 1
+#define CEB_FN_SILU 2
+#define CEB_FN_GELU 3      /* x/2 (1 + erf(x / sqrt 2)) */
+#define CEB_FN_GELU_TANH 4 /* x/2 (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) */
+CEB_API int ceb_linear_fused(const ceb_linear* lin, const void* d_x, int64_t x_stride, int m, const float* d_bias,
+                             int act, const void* d_residual, int residual_dtype, int64_t residual_stride,
+                             int out_dtype, void* d_out, int64_t out_stride, void* stream);
 CEB_API void ceb_linear_free(ceb_linear* lin);
 
 /*
