@@ -106,6 +106,11 @@ int ceb_make_tmap_2d_sw(CUtensorMap* map, const void* base, int elem_bytes, uint
 int ceb_make_tmap_2d_f16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t row_stride_bytes,
                          uint32_t box_inner, uint32_t box_rows);
 
+// 16-bit values [rows][heads][head_dim] (strides in elements, multiples of 8) in boxes of 64
+// values x box_heads x box_rows, 128-byte swizzle; values past head_dim read as zero.
+int ceb_make_tmap_heads(CUtensorMap* map, const void* base, bool bf16, int head_dim, int heads, int64_t rows,
+                        int64_t head_stride, int64_t row_stride, int box_heads, int box_rows);
+
 // kernels (launchers return 0 or an error code)
 int ceb_gemm_launch(const ceb_wplane& w, const void* act_f16, int act_rows_capacity, const ceb_gemm_args& a,
                     cudaStream_t stream, int max_ctas = 0);

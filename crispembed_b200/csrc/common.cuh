@@ -100,6 +100,36 @@ CEB_DEV void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int
         "l"(map), "r"(bar), "r"(x), "r"(y)
         : "memory");
 }
+CEB_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+// Ask for a block of this grid that has not started yet: the 16-byte answer arrives at `dst`
+// and counts on `bar`.  After an answer that names none, no more may be asked for.
+CEB_DEV void next_block_request(uint32_t dst, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     dst),
+                 "r"(bar)
+                 : "memory");
+}
+// The x index of the block that the answer at `src` names, or -1.
+CEB_DEV int next_block_answer(uint32_t src) {
+    uint32_t ok, x = 0;
+    asm volatile(
+        "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+        "ld.shared.b128 h, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+        : "=r"(ok), "=r"(x)
+        : "r"(src)
+        : "memory");
+    return ok ? (int)x : -1;
+}
 // contiguous global -> shared bulk copy (16-byte aligned addresses, size a multiple of 16)
 CEB_DEV void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),

@@ -124,6 +124,21 @@ int ceb_make_tmap_2d_sw(CUtensorMap* map, const void* base, int elem_bytes, uint
     return 0;
 }
 
+int ceb_make_tmap_heads(CUtensorMap* map, const void* base, bool bf16, int head_dim, int heads, int64_t rows,
+                        int64_t head_stride, int64_t row_stride, int box_heads, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return ceb_set_error(3, "cuTensorMapEncodeTiled unavailable");
+    cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)rows};
+    cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                    const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return ceb_set_error(3, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return 0;
+}
+
 int ceb_make_tmap_2d_f16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t row_stride_bytes,
                          uint32_t box_inner, uint32_t box_rows) {
     return ceb_make_tmap_2d(map, base, 2, inner, rows, row_stride_bytes, box_inner, box_rows, true);
