@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import List, Optional, Sequence, Union
 
 import numpy as np
@@ -48,6 +49,10 @@ class _AttnParams(ctypes.Structure):
            ("softcap", ctypes.c_float), ("window_left", ctypes.c_int), ("window_right", ctypes.c_int)]
         + [(n, ctypes.c_void_p) for n in ("d_prefix", "d_doc_q", "d_doc_k", "d_slopes", "d_rel_bias")]
         + [("rel_bias_radius", ctypes.c_int)])
+
+
+# ceb_attn_params as bytes (the same layout; packing is quicker than filling the structure)
+_ATTN_PARAMS = struct.Struct("@9i4x8q2P2f2i5Pi4x")
 
 
 def load_library(path: Optional[str] = None):
@@ -118,7 +123,7 @@ def load_library(path: Optional[str] = None):
         "ceb_linear_fused": ([vp, vp, ctypes.c_int64, ctypes.c_int, vp, ctypes.c_int, vp, ctypes.c_int, ctypes.c_int64,
                               ctypes.c_int, vp, ctypes.c_int64, vp], ctypes.c_int),
         "ceb_linear_free": ([vp], None),
-        "ceb_attention_masked": ([ctypes.POINTER(_AttnParams), vp, vp, vp, vp, vp], ctypes.c_int),
+        "ceb_attention_masked": ([vp, vp, vp, vp, vp, vp], ctypes.c_int),
         "ceb_rope_create": ([ctypes.c_int, ctypes.c_double, ctypes.c_int, ctypes.c_double, ctypes.c_int,
                              ctypes.c_double, ctypes.c_double], vp),
         "ceb_rope_forward": ([vp, vp, vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64,
@@ -162,28 +167,43 @@ def _ptr(t) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _need(ok: bool, what: str):
-    if not ok:
-        raise CrispEmbedError(what)
+# The operators of the attention block are called once a layer and token: their wrappers test
+# plain conditions and build messages only to raise them.
+_block = None
 
 
-def _on(x, what: str, **tensors):
-    """The device of `x` (a CUDA tensor); every other tensor given must lie there too."""
-    _need(x.is_cuda, f"{what}: CUDA tensors expected")
-    for name, t in tensors.items():
-        _need(t is None or t.device == x.device, f"{what}: {name} is on {getattr(t, 'device', None)}, not {x.device}")
-    return x.device
+def _block_state():
+    """(torch, {dtype: CEB_ACT_*}, library), looked up once."""
+    global _block
+    if _block is None:
+        import torch
+        _block = (torch, {torch.float32: ACT_F32, torch.bfloat16: ACT_BF16, torch.float16: ACT_F16}, load_library())
+    return _block
+
+
+def _same_device(what: str, x, tensors):
+    """The device index of `x`, on which every other tensor (None allowed) must lie too."""
+    dev = x.get_device()
+    if dev < 0:
+        raise CrispEmbedError(f"{what}: CUDA tensors expected")
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise CrispEmbedError(f"{what}: a tensor on {t.device}, not on {x.device}")
+    return dev
 
 
 def _vector(t, dtype, n: int, what: str):
     """`t` (None allowed) is a contiguous vector of n values of `dtype`."""
-    _need(t is None or (t.dtype == dtype and t.numel() == n and t.is_contiguous()),
-          f"{what}: {n} contiguous values of {dtype} expected")
+    if t is not None and (t.dtype != dtype or t.numel() != n or not t.is_contiguous()):
+        raise CrispEmbedError(f"{what}: {n} contiguous values of {dtype} expected")
 
 
-def _act_types():
-    import torch
-    return {torch.float32: ACT_F32, torch.bfloat16: ACT_BF16, torch.float16: ACT_F16}
+def _call_on(torch, dev: int, stream, call):
+    """call(stream pointer) with device `dev` current, on its current stream unless one is given."""
+    if torch.cuda.current_device() == dev:
+        return call(torch.cuda.current_stream(dev).cuda_stream if stream is None else int(stream))
+    with torch.cuda.device(dev):
+        return call(torch.cuda.current_stream(dev).cuda_stream if stream is None else int(stream))
 
 
 class CrispEmbed:
@@ -466,24 +486,27 @@ class Linear:
         x: [m, k] fp16; residual, out: [m, n_out] in fp32, fp16 or bf16; rows may be strided.
         act: "none", "relu", "silu", "gelu" or "gelu_tanh".  out (default: new, of out_dtype or
         fp16) may be the residual.  Runs on x's device and its current stream."""
-        import torch
-        types = _act_types()
-        _need(act in ACTIVATIONS, f"fused: activation {act!r}: one of {', '.join(ACTIVATIONS)}")
-        _need(x.dim() == 2 and x.shape[1] == self.k and x.dtype == torch.float16 and x.stride(1) == 1,
-              f"fused: x must be fp16 [rows, {self.k}] with contiguous rows")
-        dev = _on(x, "fused", bias=bias, residual=residual, out=out)
-        _vector(bias, torch.float32, self.n_out, "fused: bias")
+        torch, types, lib = _block_state()
+        m, n = x.shape[0], self.n_out
+        if act not in ACTIVATIONS:
+            raise CrispEmbedError(f"fused: activation {act!r}: one of {', '.join(ACTIVATIONS)}")
+        if x.dim() != 2 or x.shape[1] != self.k or x.dtype != torch.float16 or x.stride(1) != 1:
+            raise CrispEmbedError(f"fused: x must be fp16 [rows, {self.k}] with contiguous rows")
+        dev = _same_device("fused", x, (bias, residual, out))
+        _vector(bias, torch.float32, n, "fused: bias")
         if out is None:
-            out = torch.empty((x.shape[0], self.n_out), dtype=out_dtype or torch.float16, device=dev)
-        for name, t in (("residual", residual), ("out", out)):
-            _need(t is None or (t.dtype in types and t.shape == (x.shape[0], self.n_out) and t.stride(1) == 1),
-                  f"fused: {name} must be [{x.shape[0]}, {self.n_out}] in fp32, fp16 or bf16 with contiguous rows")
-        _need(out_dtype is None or out.dtype == out_dtype, "fused: out is not of out_dtype")
-        with torch.cuda.device(dev):
-            _check(self._lib.ceb_linear_fused(
-                self._h, x.data_ptr(), x.stride(0), x.shape[0], _ptr(bias), ACTIVATIONS[act], _ptr(residual),
-                0 if residual is None else types[residual.dtype], 0 if residual is None else residual.stride(0),
-                types[out.dtype], out.data_ptr(), out.stride(0), _stream_ptr(stream)), "ceb_linear_fused")
+            out = torch.empty((m, n), dtype=out_dtype or torch.float16, device=x.device)
+        elif out_dtype is not None and out.dtype != out_dtype:
+            raise CrispEmbedError("fused: out is not of out_dtype")
+        for t in (out,) if residual is None else (out, residual):
+            if t.dtype not in types or t.shape != (m, n) or t.stride(1) != 1:
+                raise CrispEmbedError(f"fused: residual and out must be [{m}, {n}] in fp32, fp16 or bf16 with contiguous rows")
+        res = (None, 0, 0) if residual is None else (residual.data_ptr(), types[residual.dtype], residual.stride(0))
+        rc = _call_on(torch, dev, stream, lambda st: lib.ceb_linear_fused(
+            self._h, x.data_ptr(), x.stride(0), m, None if bias is None else bias.data_ptr(), ACTIVATIONS[act], *res,
+            types[out.dtype], out.data_ptr(), out.stride(0), st))
+        if rc:
+            _check(rc, "ceb_linear_fused")
         return out
 
     def close(self):
@@ -550,44 +573,57 @@ def attention_masked(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, max_
     int32 document numbers (doc_k default: doc_q).  slopes: fp32 [n_head], or rel_bias: fp32
     [n_head, 2 R + 1].  Returns out, [q_rows, n_head, head_dim]; rows of no sequence are not
     written.  Runs on q's device and its current stream."""
-    import torch
-    types = {t: c for t, c in _act_types().items() if t != torch.float32}
-    _need(q.dtype in types and k.dtype == q.dtype and v.dtype == q.dtype, "attention_masked: q, k, v in fp16 or bf16")
-    _need(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape and k.shape[2] == q.shape[2],
-          "attention_masked: q [rows, heads, head_dim], k and v [keys, key heads, head_dim] expected")
-    _need(all(t.stride(2) == 1 for t in (q, k, v)), "attention_masked: the values of a head must be contiguous")
-    cu_k = cu_q if cu_k is None else cu_k
-    doc_k = doc_q if doc_k is None else doc_k
-    dev = _on(q, "attention_masked", k=k, v=v, cu_q=cu_q, cu_k=cu_k, prefix=prefix, doc_q=doc_q, doc_k=doc_k,
-              slopes=slopes, rel_bias=rel_bias, out=out)
+    torch, types, lib = _block_state()
+    dtype = q.dtype
+    if dtype not in types or dtype == torch.float32 or k.dtype != dtype or v.dtype != dtype:
+        raise CrispEmbedError("attention_masked: q, k, v in fp16 or bf16, all alike, expected")
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2]:
+        raise CrispEmbedError("attention_masked: q [rows, heads, head_dim], k and v [keys, key heads, head_dim] expected")
+    (qr, qh, q1), (kr, kh, k1), (vr, vh, v1) = q.stride(), k.stride(), v.stride()
+    if q1 != 1 or k1 != 1 or v1 != 1:
+        raise CrispEmbedError("attention_masked: the values of a head must be contiguous")
+    if cu_k is None:
+        cu_k = cu_q
+    if doc_k is None:
+        doc_k = doc_q
+    dev = _same_device("attention_masked", q, (k, v, cu_q, cu_k, prefix, doc_q, doc_k, slopes, rel_bias, out))
     rows, n_head, hd = q.shape
-    n = cu_q.numel() - 1
-    _need(n >= 0, "attention_masked: row offsets expected")
-    _vector(cu_q, torch.int32, n + 1, "attention_masked: cu_q")
-    _vector(cu_k, torch.int32, n + 1, "attention_masked: cu_k")
-    _vector(prefix, torch.int32, n, "attention_masked: prefix")
-    _vector(doc_q, torch.int32, rows, "attention_masked: doc_q")
-    _vector(doc_k, torch.int32, k.shape[0], "attention_masked: doc_k")
-    _vector(slopes, torch.float32, n_head, "attention_masked: slopes")
+    keys, n = k.shape[0], cu_q.numel() - 1
+    if n < 0:
+        raise CrispEmbedError("attention_masked: row offsets expected")
+    i32, f32 = torch.int32, torch.float32
+    _vector(cu_q, i32, n + 1, "attention_masked: cu_q")
+    _vector(cu_k, i32, n + 1, "attention_masked: cu_k")
+    _vector(prefix, i32, n, "attention_masked: prefix")
+    _vector(doc_q, i32, rows, "attention_masked: doc_q")
+    _vector(doc_k, i32, keys, "attention_masked: doc_k")
+    _vector(slopes, f32, n_head, "attention_masked: slopes")
     radius = 0
     if rel_bias is not None:
-        _need(rel_bias.dim() == 2 and rel_bias.shape[1] % 2 == 1, "attention_masked: rel_bias [heads, 2 R + 1] expected")
+        if rel_bias.dim() != 2 or rel_bias.shape[1] % 2 != 1:
+            raise CrispEmbedError("attention_masked: rel_bias [heads, 2 R + 1] expected")
         radius = rel_bias.shape[1] // 2
-        _vector(rel_bias, torch.float32, n_head * (2 * radius + 1), "attention_masked: rel_bias")
-    left, right = window
-    longest = [int((c[1:] - c[:-1]).max().item()) if given is None and n else given or 0
-               for c, given in ((cu_q, max_q), (cu_k, max_k))]
+        _vector(rel_bias, f32, n_head * (2 * radius + 1), "attention_masked: rel_bias")
+    if max_q is None:
+        max_q = int((cu_q[1:] - cu_q[:-1]).max().item()) if n else 0
+    if max_k is None:
+        max_k = int((cu_k[1:] - cu_k[:-1]).max().item()) if n else 0
     if out is None:
-        out = torch.empty((rows, n_head, hd), dtype=q.dtype, device=dev)
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1,
-          "attention_masked: out must have q's shape and type, the values of a head contiguous")
-    p = _AttnParams(types[q.dtype], n_head, k.shape[1], hd, n, rows, k.shape[0], longest[0], longest[1],
-                    q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0),
-                    out.stride(1), _ptr(cu_q), _ptr(cu_k), hd ** -0.5 if scale is None else scale, softcap, left, right,
-                    _ptr(prefix), _ptr(doc_q), _ptr(doc_k), _ptr(slopes), _ptr(rel_bias), radius)
-    with torch.cuda.device(dev):
-        _check(load_library().ceb_attention_masked(ctypes.byref(p), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                                   out.data_ptr(), _stream_ptr(stream)), "ceb_attention_masked")
+        out = torch.empty((rows, n_head, hd), dtype=dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != dtype:
+        raise CrispEmbedError("attention_masked: out must have q's shape and type")
+    rr, rh, r1 = out.stride()
+    if r1 != 1:
+        raise CrispEmbedError("attention_masked: the values of a head must be contiguous")
+    p = _ATTN_PARAMS.pack(types[dtype], n_head, k.shape[1], hd, n, rows, keys, max_q, max_k, qr, qh, kr, kh, vr, vh, rr, rh,
+                          cu_q.data_ptr(), cu_k.data_ptr(), hd ** -0.5 if scale is None else scale, softcap, window[0],
+                          window[1], 0 if prefix is None else prefix.data_ptr(), 0 if doc_q is None else doc_q.data_ptr(),
+                          0 if doc_k is None else doc_k.data_ptr(), 0 if slopes is None else slopes.data_ptr(),
+                          0 if rel_bias is None else rel_bias.data_ptr(), radius)
+    rc = _call_on(torch, dev, stream, lambda st: lib.ceb_attention_masked(p, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                                                          out.data_ptr(), st))
+    if rc:
+        _check(rc, "ceb_attention_masked")
     return out
 
 
@@ -600,7 +636,8 @@ class Rope:
     def __init__(self, rot_dim: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0,
                  context: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0):
         """The plan lies on the current device.  scaling: "none", "linear", "ntk" or "yarn"."""
-        _need(scaling in ROPE_SCALINGS, f"Rope: scaling {scaling!r}: one of {', '.join(ROPE_SCALINGS)}")
+        if scaling not in ROPE_SCALINGS:
+            raise CrispEmbedError(f"Rope: scaling {scaling!r}: one of {', '.join(ROPE_SCALINGS)}")
         self._h = None
         self._lib = load_library()
         self.rot_dim = rot_dim
@@ -614,25 +651,32 @@ class Rope:
         """x: [rows, heads, head_dim] in fp32, fp16 or bf16, rows and heads strided at will.  Positions:
         int32 [rows], or the rows' places in the sequences of cu_seqlens (int32) plus pos_offset.
         out (default: new) may be x.  Runs on x's device and its current stream."""
-        import torch
-        types = _act_types()
-        _need(x.dim() == 3 and x.dtype in types and (x.stride(2) == 1 or x.shape[2] == 1),
-              "Rope: x must be [rows, heads, head_dim] in fp32, fp16 or bf16, the values of a head contiguous")
-        dev = _on(x, "Rope", out=out, positions=positions, cu_seqlens=cu_seqlens)
-        _need(positions is not None or cu_seqlens is not None, "Rope: positions or cu_seqlens must be given")
-        _vector(positions, torch.int32, x.shape[0], "Rope: positions")
+        torch, types, lib = _block_state()
+        dtype = x.dtype
+        if x.dim() != 3 or dtype not in types:
+            raise CrispEmbedError("Rope: x must be [rows, heads, head_dim] in fp32, fp16 or bf16")
+        dev = _same_device("Rope", x, (out, positions, cu_seqlens))
+        rows, heads, hd = x.shape
+        if positions is None and cu_seqlens is None:
+            raise CrispEmbedError("Rope: positions or cu_seqlens must be given")
+        n = 0
+        _vector(positions, torch.int32, rows, "Rope: positions")
         if cu_seqlens is not None:
-            _vector(cu_seqlens, torch.int32, cu_seqlens.numel(), "Rope: cu_seqlens")
+            n = cu_seqlens.numel() - 1
+            _vector(cu_seqlens, torch.int32, n + 1, "Rope: cu_seqlens")
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        _need(out.shape == x.shape and out.dtype == x.dtype and out.stride(2) == 1,
-              "Rope: out must have x's shape and type, the values of a head contiguous")
-        n = 0 if cu_seqlens is None else cu_seqlens.numel() - 1
-        with torch.cuda.device(dev):
-            _check(self._lib.ceb_rope_forward(self._h, x.data_ptr(), out.data_ptr(), types[x.dtype], x.shape[0],
-                                              x.shape[1], x.shape[2], x.stride(0), x.stride(1), out.stride(0),
-                                              out.stride(1), int(interleaved), _ptr(positions), _ptr(cu_seqlens), n,
-                                              pos_offset, _stream_ptr(stream)), "ceb_rope_forward")
+            out = torch.empty((rows, heads, hd), dtype=dtype, device=x.device)
+        elif out.shape != x.shape or out.dtype != dtype:
+            raise CrispEmbedError("Rope: out must have x's shape and type")
+        (xr, xh, x1), (rr, rh, r1) = x.stride(), out.stride()
+        if (x1 != 1 or r1 != 1) and hd > 1:
+            raise CrispEmbedError("Rope: the values of a head must be contiguous")
+        rc = _call_on(torch, dev, stream, lambda st: lib.ceb_rope_forward(
+            self._h, x.data_ptr(), out.data_ptr(), types[dtype], rows, heads, hd, xr, xh, rr, rh, interleaved,
+            None if positions is None else positions.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(), n,
+            pos_offset, st))
+        if rc:
+            _check(rc, "ceb_rope_forward")
         return out
 
     def close(self):

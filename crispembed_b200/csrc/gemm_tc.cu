@@ -39,6 +39,7 @@
 // stage; quantized planes are dequantized in shared memory as here.
 #include <cstdio>
 #include <cstdlib>
+#include <type_traits>
 
 #include "../../include/ceb_ops.h"
 #include "ceb_internal.h"
@@ -290,24 +291,28 @@ CEB_DEV f32x2 gelu_as2(f32x2 x) {
 // is the same with 2 sqrt(2/pi) (x + 0.044715 x^3) in the exponent, since
 // (1 + tanh u) / 2 = 1 / (1 + exp(-2u)).  Exponential and reciprocal are the MUFU
 // approximations (relative error ~2^-22, below the fp32 sums in front of them).
-CEB_DEV float ex_act(float x, int act) {
-    if (act == CEB_FN_GELU) return gelu_as(x);
-    if (act == CEB_FN_RELU) return x < 0.0f ? 0.0f : x;  // NaN stays
-    if (act == CEB_FN_NONE) return x;
+template <int ACT>
+CEB_DEV float ex_act1(float x) {
+    if (ACT == CEB_FN_GELU) return gelu_as(x);
+    if (ACT == CEB_FN_RELU) return x < 0.0f ? 0.0f : x;  // NaN stays
+    if (ACT == CEB_FN_NONE) return x;
     constexpr float kL = 1.4426950408889634f, kG = 2.0f * 0.79788456080286536f;
-    const float u = act == CEB_FN_SILU ? x : kG * fmaf(0.044715f * x * x, x, x);
+    const float u = ACT == CEB_FN_SILU ? x : kG * fmaf(0.044715f * x * x, x, x);
     return x * rcp_approx(1.0f + ex2_approx(-kL * u));
 }
-// four consecutive values of type CEB_ACT_* at element `i` of `p` (aligned to four values)
-CEB_DEV float4 load4(const void* p, int type, int64_t i) {
-    if (type == CEB_ACT_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-    if (type == CEB_ACT_BF16)
-        return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                           __uint_as_float(u.y & 0xffff0000u));
-    const float2 a = __half22float2(u32_as_h2(u.x)), b = __half22float2(u32_as_h2(u.y));
-    return make_float4(a.x, a.y, b.x, b.y);
+template <int ACT>
+CEB_DEV void ex_act_all(float* x) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = ex_act1<ACT>(x[j]);
 }
+// 32 values: one branch for all
+CEB_DEV void ex_act(float* x, int act) {
+    if (act == CEB_FN_SILU) ex_act_all<CEB_FN_SILU>(x);
+    else if (act == CEB_FN_GELU) ex_act_all<CEB_FN_GELU>(x);
+    else if (act == CEB_FN_GELU_TANH) ex_act_all<CEB_FN_GELU_TANH>(x);
+    else if (act == CEB_FN_RELU) ex_act_all<CEB_FN_RELU>(x);
+}
+// one value of type CEB_ACT_* at element `i` of `p`
 CEB_DEV float load1(const void* p, int type, int64_t i) {
     if (type == CEB_ACT_F32) return static_cast<const float*>(p)[i];
     if (type == CEB_ACT_F16) return __half2float(static_cast<const __half*>(p)[i]);
@@ -531,9 +536,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
                     x[j] = __uint_as_float(v[j]) + bv;
-                    if (EX) x[j] = ex_act(x[j], a.act);
-                    else if (gelu) x[j] = gelu_as(x[j]);
+                    if (!EX && gelu) x[j] = gelu_as(x[j]);
                 }
+                if (EX) ex_act(x, a.act);
                 const int lim = ti.rows - c0;
                 if (EX && a.res) {
 #pragma unroll
@@ -645,14 +650,15 @@ struct Smem {
 
 // Shared-memory plan and barrier indices for PS A+B stages and PR raw weight stages
 // (PR = 0: fp16 weights loaded by TMA, no raw stage).
-template <int PS_, int PR_, int NSLOT_, int KS_ = 1>
+template <int PS_, int PR_, int NSLOT_, int KS_ = 1, int RSLOT_ = 0>
 struct Lay {
     static constexpr int PS = PS_, PR = PR_;
     static constexpr int KS = KS_;                              // 64-wide K atoms per A+B stage
     static constexpr int STAGE_T = KS * STAGE;
     static constexpr int NSLOT = NSLOT_;                        // staging slots per epilogue warp
-    static constexpr int STAGING = 4 * EPI_WG * NSLOT * SLOT;
-    static constexpr int NB = 2 * PS + 4 + 1 + 2 * PR + PS + 2;
+    static constexpr int RSLOT = RSLOT_;                        // residual slots per epilogue warp (extended epilogue)
+    static constexpr int STAGING = 4 * EPI_WG * (NSLOT + RSLOT) * SLOT;
+    static constexpr int NB = 2 * PS + 4 + 1 + 2 * PR + PS + 2 + 4 * EPI_WG * RSLOT;
     static constexpr int SIG_BYTES = (PS + 2 + 1) * SIG;  // sinks for FULL[s], ACC_EMPTY[b] + one source
     static constexpr size_t SMEM = 1024 + (size_t)PS * STAGE_T + (size_t)PR * RAW_STAGE + STAGING + SIG_BYTES +
                                    NB * 8 + 16 + 3 * (MAXG + 1) * 4;
@@ -670,6 +676,7 @@ struct Lay {
     static CEB_DEV int B_RAW_EMPTY(int r) { return 2 * PS + 5 + PR + r; }
     static CEB_DEV int B_W_FULL(int s) { return 2 * PS + 5 + 2 * PR + s; }    // rank 1 only
     static CEB_DEV int B_ACC_FREE(int b) { return 3 * PS + 5 + 2 * PR + b; }  // rank 1 only
+    static CEB_DEV int B_RES(int ew, int b) { return 3 * PS + 7 + 2 * PR + RSLOT * ew + b; }  // residual bytes
 
     static CEB_DEV Smem carve(uint8_t* base) {
         Smem s;
@@ -707,10 +714,27 @@ struct Lay {
 #ifndef CEB_PAIR_KS_F16
 #define CEB_PAIR_KS_F16 2
 #endif
-// quantized weights: 4 A+B stages + 4 raw stages; fp16 weights: the raw bytes become more A+B stages
+// quantized weights: 4 A+B stages + 4 raw stages; fp16 weights: the raw bytes become more A+B stages.
+// The extended epilogue takes room for the residual's slots: fp16 planes run five one-atom
+// stages and one slot.  768 -> 768 at M = 70,825 with an fp16 residual: 89.7 us; four stages and
+// two slots 90.9, three and three 95.4; residual rows read by their threads instead 131 us.
+#ifndef CEB_EX_PS
+#define CEB_EX_PS 5
+#endif
+#ifndef CEB_EX_RS
+#define CEB_EX_RS 1
+#endif
+template <int FMT, bool EX>
+struct LayOf_ {
+    using type = Lay<FMT == CEB_W_F16 ? CEB_PAIR_PS_F16 : 4, FMT == CEB_W_F16 ? 0 : 4,
+                     FMT == CEB_W_F16 ? CEB_PAIR_SLOTS_F16 : 1, FMT == CEB_W_F16 ? CEB_PAIR_KS_F16 : 1>;
+};
 template <int FMT>
-using LayOf = Lay<FMT == CEB_W_F16 ? CEB_PAIR_PS_F16 : 4, FMT == CEB_W_F16 ? 0 : 4, FMT == CEB_W_F16 ? CEB_PAIR_SLOTS_F16 : 1,
-                  FMT == CEB_W_F16 ? CEB_PAIR_KS_F16 : 1>;
+struct LayOf_<FMT, true> {
+    using type = Lay<FMT == CEB_W_F16 ? CEB_EX_PS : 3, FMT == CEB_W_F16 ? 0 : 4, 1, 1, FMT == CEB_W_F16 ? CEB_EX_RS : 1>;
+};
+template <int FMT, bool EX>
+using LayOf = typename LayOf_<FMT, EX>::type;
 
 struct Tile {
     int g, fp, row0, rows;  // group, feature-pair tile, first token of the pair tile, tokens in it (<= 256)
@@ -770,6 +794,35 @@ CEB_DEV void epi_math(uint32_t (&v)[32], const float* bias, bool gelu) {
 
 }  // namespace pair
 
+// Adds the residual of 32 columns, `part` of the warp's slot (rows of 128 B, 128-byte swizzle,
+// 16-bit types: part 0 or 1 of the row), to the row that this lane holds.
+CEB_DEV void ex_add(float* x, const uint8_t* slot, int lane, int type, int part) {
+    if (type == CEB_ACT_F32) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float4 u = *reinterpret_cast<const float4*>(slot + lane * 128 + ((k ^ (lane & 7)) << 4));
+            x[4 * k] += u.x;
+            x[4 * k + 1] += u.y;
+            x[4 * k + 2] += u.z;
+            x[4 * k + 3] += u.w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint4 u = *reinterpret_cast<const uint4*>(slot + lane * 128 + (((k + 4 * part) ^ (lane & 7)) << 4));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = type == CEB_ACT_BF16
+                                 ? make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u))
+                                 : __half22float2(u32_as_h2(w[j]));
+            x[8 * k + 2 * j] += f.x;
+            x[8 * k + 2 * j + 1] += f.y;
+        }
+    }
+}
+
 // Warps of the pair kernel: 4 control warps, the dequant warpgroups (quantized planes
 // only) and the epilogue warpgroups.  With fp16 planes the block has no dequant warps
 // (384 threads), so each thread may hold up to 168 registers instead of 102: fc1 + GELU
@@ -783,13 +836,14 @@ struct PairWarps {
 template <int FMT, bool EX>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<FMT>::THREADS, 1)
     ceb_gemm_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap omap,
-                         const __grid_constant__ CUtensorMap wmap, const ceb_wplane w, const ceb_gemm_args a) {
+                         const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap rmap, const ceb_wplane w,
+                         const ceb_gemm_args a) {
     using namespace pair;
     // fp16 weight blocks are already the MMA's swizzled image: both CTAs load them with
     // the pair TMA straight into the weight stage, counted on the leader's FULL barrier
     // (no raw stage, no dequant warps, no relayed signal).
     constexpr bool kTmaW = FMT == CEB_W_F16;
-    using L = LayOf<FMT>;
+    using L = LayOf<FMT, EX>;
     constexpr int PS = L::PS, PR = L::PR, NB = L::NB;
     extern __shared__ uint8_t smem_raw[];
     const Smem SH = L::carve(smem_raw);
@@ -835,6 +889,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<FMT>::THRE
         tma_prefetch_desc(&xmap);
         tma_prefetch_desc(&omap);
         if (kTmaW) tma_prefetch_desc(&wmap);
+        if (EX && a.res) tma_prefetch_desc(&rmap);
     }
     if (warp == 1) {
         tmem_alloc_pair(smem_u32(SH.tmem_slot), TMEM_COLS);
@@ -1041,6 +1096,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<FMT>::THRE
         const bool gelu = !EX && (a.epi & CEB_EPI_GELU) != 0;
         constexpr int NSLOT = L::NSLOT;
         uint32_t lt = 0, nstore = 0;
+        // Residual chunks (128 bytes a row) come by TMA, RSLOT of them ahead of their use, across
+        // the tiles' ends: a row's loads by its own thread would take a sector each.
+        constexpr int RSLOT = L::RSLOT > 0 ? L::RSLOT : 1;
+        uint8_t* rslots = SH.staging + (size_t)(4 * EPI_WG * NSLOT + ew * RSLOT) * SLOT;
+        uint32_t r_used = 0, r_asked = 0;
+        const int r_cols = EX && a.res_type == CEB_ACT_F32 ? 32 : 64, r_chunks = 128 / r_cols;
+        int r_tile = pair_id, r_next = 0;  // the tile and chunk to ask for next
+        auto ask_residual = [&] {
+            while (r_tile < total) {
+                const Tile rt = pair::decode(SH, G, n_fp, r_tile);
+                if (rt.rows - TOK * (int)rank - 32 * q > 0) {
+                    const int b = (int)(r_asked % RSLOT);
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(bar(L::B_RES(ew, b)), SLOT);
+                        tma_load_2d(smem_u32(rslots + b * SLOT), &rmap, bar(L::B_RES(ew, b)),
+                                    rt.fp * FEAT + 128 * wg + r_cols * r_next, rt.row0 + TOK * (int)rank + 32 * q);
+                    }
+                    __syncwarp();
+                    ++r_asked;
+                    if (++r_next == r_chunks) r_next = 0, r_tile += n_pairs;
+                    return;
+                }
+                r_tile += n_pairs;
+            }
+        };
+        if constexpr (EX) {
+            if (a.res)
+                for (int b = 0; b < RSLOT; ++b) ask_residual();
+        }
         for (int t = pair_id; t < total; t += n_pairs, ++lt) {
             const Tile ti = pair::decode(SH, G, n_fp, t);
             const int ab = lt & 1;
@@ -1053,6 +1137,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<FMT>::THRE
             const float* bias = (a.epi & CEB_EPI_BIAS) ? a.bias + (size_t)ti.g * a.bias_group_stride : nullptr;
             const uint32_t col0 = (uint32_t)(ab * FEAT + 128 * wg);
             const int chunk_cols = f16 ? 64 : 32;
+            if constexpr (EX) {
+                // 32 columns at a time
+                uint8_t* slot = SH.staging + (size_t)ew * SLOT;
+                const bool full = lim >= 32;
+                bool lost = false;  // a residual chunk did not come
+                for (int c = 0; c < 4; ++c) {
+                    if (lim <= 0) break;
+                    uint32_t v[32];
+                    tmem_ld32(tmem + lane_addr + col0 + (uint32_t)(32 * c), v);
+                    tmem_ld_wait();
+                    epi_math<kTmaW>(v, bias ? bias + f_base + 32 * c : nullptr, false);
+                    float* x = reinterpret_cast<float*>(v);
+                    ex_act(x, a.act);
+                    if (a.res) {
+                        const int b = (int)(r_used % RSLOT), rp = a.res_type == CEB_ACT_F32 ? 0 : c & 1;
+                        lost = !__all_sync(0xffffffffu, wait_at(L::B_RES(ew, b), (r_used / RSLOT) & 1, CEB_DEVERR_TIMEOUT_EPI));
+                        if (lost) break;
+                        ex_add(x, rslots + b * SLOT, lane, a.res_type, rp);
+                        if (a.res_type == CEB_ACT_F32 || rp == 1) {
+                            __syncwarp();  // the slot has been read
+                            ++r_used;
+                            ask_residual();
+                        }
+                    }
+                    const int part = f16 ? c & 1 : 0;  // half of a 128-byte slot row
+                    if (full && part == 0 && nstore >= 1) {  // the slot's last store has read it
+                        if (lane == 0) bulk_wait_read<0>();
+                        __syncwarp();
+                    }
+                    if (f16) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) p[j] = pack2(x[2 * j], x[2 * j + 1], a.out_type);
+                        uint16_t* o = static_cast<uint16_t*>(a.out) + (size_t)(row + lane) * a.ldo + f_base + 32 * c;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint4 w = make_uint4(p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]);
+                            if (full)
+                                *reinterpret_cast<uint4*>(slot + lane * 128 + (((k + 4 * part) ^ (lane & 7)) << 4)) = w;
+                            else if (lane < lim)
+                                reinterpret_cast<uint4*>(o)[k] = w;
+                        }
+                    } else {
+                        float* o = static_cast<float*>(a.out) + (size_t)(row + lane) * a.ldo + f_base + 32 * c;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float4 w = make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+                            if (full)
+                                *reinterpret_cast<float4*>(slot + lane * 128 + ((k ^ (lane & 7)) << 4)) = w;
+                            else if (lane < lim)
+                                reinterpret_cast<float4*>(o)[k] = w;
+                        }
+                    }
+                    if (full && (!f16 || part == 1)) {
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_2d(&omap, smem_u32(slot), f_base + 32 * (c - part), row);
+                            bulk_commit();
+                        }
+                        ++nstore;
+                    }
+                }
+                if (lost) break;
+            } else
             for (int c0 = 0; c0 < 128; c0 += chunk_cols) {
                 if (lim <= 0) break;
                 const bool full = lim >= 32;
@@ -1101,28 +1250,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<FMT>::THRE
                         tmem_ld32(tmem + lane_addr + col0 + (uint32_t)(c0 + h), v);
                         tmem_ld_wait();
                         epi_math<kTmaW>(v, bias ? bias + f_base + c0 + h : nullptr, gelu);
-                        float* x = reinterpret_cast<float*>(v);
-                        if constexpr (EX) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) x[j] = ex_act(x[j], a.act);
-                            if (a.res && lane < lim) {
-                                const int64_t at = (int64_t)(row + lane) * a.ldr + f_base + c0 + h;
-#pragma unroll
-                                for (int j = 0; j < 32; j += 4) {
-                                    const float4 r = load4(a.res, a.res_type, at + j);
-                                    x[j] += r.x;
-                                    x[j + 1] += r.y;
-                                    x[j + 2] += r.z;
-                                    x[j + 3] += r.w;
-                                }
-                            }
-                        }
+                        const float* x = reinterpret_cast<const float*>(v);
                         if (f16) {
                             uint32_t p[16];
     #pragma unroll
                             for (int j = 0; j < 16; ++j)
-                                p[j] = EX ? pack2(x[2 * j], x[2 * j + 1], a.out_type)
-                                          : h2_as_u32(__floats2half2_rn(x[2 * j], x[2 * j + 1]));
+                                p[j] = h2_as_u32(__floats2half2_rn(x[2 * j], x[2 * j + 1]));
                             if (full) {  // 64 B = chunks 4*(h/32) .. +3 of the 128-B swizzled row
     #pragma unroll
                                 for (int c = 0; c < 4; ++c) {
@@ -1173,6 +1306,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<FMT>::THRE
             }
         }
         if (lane == 0) bulk_wait<0>();  // output stores complete before the CTA retires
+        if constexpr (EX) {  // and so do residual chunks that were asked for
+            for (; r_used < r_asked; ++r_used)
+                mbar_wait(bar(L::B_RES(ew, (int)(r_used % RSLOT))), (r_used / RSLOT) & 1, nullptr, nullptr, 0);
+        }
     }
 
     tc_fence_before();
@@ -1185,24 +1322,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<FMT>::THRE
 }
 
 template <int FMT, bool EX>
-int launch_pair(const CUtensorMap& xmap, const CUtensorMap& omap, const CUtensorMap& wmap, const ceb_wplane& w,
+int launch_pair(const CUtensorMap& xmap, const CUtensorMap& omap, const CUtensorMap& wmap, const CUtensorMap& rmap,
+                const ceb_wplane& w,
                 const ceb_gemm_args& a, int max_pairs, cudaStream_t st) {
     static int resident_of[CEB_MAX_DEVICES] = {};  // co-resident pairs, per device
     int& pairs_resident = resident_of[ceb_device_index()];
     if (!pairs_resident) {
-        if (int rc = ceb_func_smem(reinterpret_cast<const void*>(ceb_gemm_pair_kernel<FMT, EX>), pair::LayOf<FMT>::SMEM))
+        if (int rc = ceb_func_smem(reinterpret_cast<const void*>(ceb_gemm_pair_kernel<FMT, EX>), pair::LayOf<FMT, EX>::SMEM))
             return rc;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2 * ceb_num_sms(), 1, 1);
         cfg.blockDim = dim3(PairWarps<FMT>::THREADS, 1, 1);
-        cfg.dynamicSmemBytes = pair::LayOf<FMT>::SMEM;
+        cfg.dynamicSmemBytes = pair::LayOf<FMT, EX>::SMEM;
         int n = 0;  // cluster size comes from the kernel's __cluster_dims__
         CEB_CUDA_OK(cudaOccupancyMaxActiveClusters(&n, ceb_gemm_pair_kernel<FMT, EX>, &cfg));
         pairs_resident = n > 0 ? n : 1;
     }
     int pairs = pairs_resident < max_pairs ? pairs_resident : max_pairs;
     if (pairs < 1) pairs = 1;
-    ceb_gemm_pair_kernel<FMT, EX><<<2 * pairs, PairWarps<FMT>::THREADS, pair::LayOf<FMT>::SMEM, st>>>(xmap, omap, wmap, w,
+    ceb_gemm_pair_kernel<FMT, EX><<<2 * pairs, PairWarps<FMT>::THREADS, pair::LayOf<FMT, EX>::SMEM, st>>>(xmap, omap, wmap, rmap, w,
                                                                                                 a);
     CEB_CUDA_OK(cudaGetLastError());
     return 0;
@@ -1269,7 +1407,7 @@ static bool ceb_gemm_use_pairs(const ceb_wplane& w, const ceb_gemm_args& a) {
     }();
     if (forced_single) return false;
     if (w.n_out % pair::FEAT) return false;
-    if (w.format == CEB_W_F16 && (w.k / BK) % CEB_PAIR_KS_F16) return false;  // whole stages of K atoms
+    if (w.format == CEB_W_F16 && !a.ex && (w.k / BK) % CEB_PAIR_KS_F16) return false;  // whole stages of K atoms
     if ((a.epi & CEB_EPI_BIAS) &&
         ((reinterpret_cast<uintptr_t>(a.bias) & 15) || (a.offsets && (a.bias_group_stride & 3))))
         return false;
@@ -1308,7 +1446,13 @@ int ceb_gemm_launch(const ceb_wplane& w, const void* act_f16, int act_rows, cons
         int max_pairs = ceb_num_sms() / 2;
         if (max_ctas > 0 && max_ctas / 2 < max_pairs) max_pairs = max_ctas / 2 > 0 ? max_ctas / 2 : 1;
         if (bound < max_pairs) max_pairs = (int)bound;
-        CUtensorMap wmap = {};
+        CUtensorMap wmap = {}, rmap = {};
+        if (a.ex && a.res) {  // residual: 32-row boxes of 128 bytes a row
+            const int rsz = a.res_type == CEB_ACT_F32 ? 4 : 2;
+            mrc = ceb_make_tmap_2d(&rmap, a.res, rsz, (uint64_t)w.n_out, (uint64_t)a.m_rows, (uint64_t)a.ldr * rsz,
+                                   128 / rsz, 32, true);
+            if (mrc) return mrc;
+        }
         if (w.format == CEB_W_F16) {  // the plane as [blocks * 128 rows, 64] fp16, blocks already swizzled
             const uint64_t blocks = (uint64_t)w.n_groups * (w.n_out / BM) * (w.k / BK);
             mrc = ceb_make_tmap_2d(&wmap, w.q, 2, (uint64_t)BK, blocks * BM, (uint64_t)BK * 2, BK, BM, false);
@@ -1316,9 +1460,9 @@ int ceb_gemm_launch(const ceb_wplane& w, const void* act_f16, int act_rows, cons
         }
         int rc = 0;
         switch (w.format) {
-            case CEB_W_Q8_0: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = a.ex ? launch_pair<CEB_W_Q8_0, true>(map, omap, wmap, w, a, max_pairs, stream) : launch_pair<CEB_W_Q8_0, false>(map, omap, wmap, w, a, max_pairs, stream)); break;
-            case CEB_W_Q4_K: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = a.ex ? launch_pair<CEB_W_Q4_K, true>(map, omap, wmap, w, a, max_pairs, stream) : launch_pair<CEB_W_Q4_K, false>(map, omap, wmap, w, a, max_pairs, stream)); break;
-            case CEB_W_F16: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = a.ex ? launch_pair<CEB_W_F16, true>(map, omap, wmap, w, a, max_pairs, stream) : launch_pair<CEB_W_F16, false>(map, omap, wmap, w, a, max_pairs, stream)); break;
+            case CEB_W_Q8_0: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = a.ex ? launch_pair<CEB_W_Q8_0, true>(map, omap, wmap, rmap, w, a, max_pairs, stream) : launch_pair<CEB_W_Q8_0, false>(map, omap, wmap, rmap, w, a, max_pairs, stream)); break;
+            case CEB_W_Q4_K: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = a.ex ? launch_pair<CEB_W_Q4_K, true>(map, omap, wmap, rmap, w, a, max_pairs, stream) : launch_pair<CEB_W_Q4_K, false>(map, omap, wmap, rmap, w, a, max_pairs, stream)); break;
+            case CEB_W_F16: CEB_LAUNCH(a.prof_cat, stream, flops, bytes, rc = a.ex ? launch_pair<CEB_W_F16, true>(map, omap, wmap, rmap, w, a, max_pairs, stream) : launch_pair<CEB_W_F16, false>(map, omap, wmap, rmap, w, a, max_pairs, stream)); break;
             default: return ceb_set_error(2, "gemm: unknown weight format %d", w.format);
         }
         return rc;
