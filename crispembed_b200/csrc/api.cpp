@@ -954,17 +954,17 @@ extern "C" int ceb_linear_fused(const ceb_linear* L, const void* d_x, int64_t x_
     a.bias = d_bias;
     a.err = err;
     a.ldx = x_stride;
-    if (!d_residual && out_dtype != CEB_ACT_BF16 && (act == CEB_FN_NONE || act == CEB_FN_GELU)) {
+    a.act = act;
+    a.out_type = out_dtype;
+    a.res = d_residual;
+    a.res_type = residual_dtype;
+    a.ldr = residual_stride;
+    if (ceb_linear_is_few(L->w, m)) return ceb_linear_few(L->w, d_x, a, static_cast<cudaStream_t>(stream));
+    if (!d_residual && out_dtype != CEB_ACT_BF16 && (act == CEB_FN_NONE || act == CEB_FN_GELU))
         // what ceb_linear_forward computes
         a.epi |= (out_dtype == CEB_ACT_F16 ? CEB_EPI_F16_OUT : 0) | (act == CEB_FN_GELU ? CEB_EPI_GELU : 0);
-    } else {
+    else
         a.ex = true;
-        a.act = act;
-        a.out_type = out_dtype;
-        a.res = d_residual;
-        a.res_type = residual_dtype;
-        a.ldr = residual_stride;
-    }
     return ceb_gemm_launch(L->w, d_x, m, a, static_cast<cudaStream_t>(stream));
 }
 

@@ -114,6 +114,10 @@ int ceb_make_tmap_heads(CUtensorMap* map, const void* base, bool bf16, int head_
 // kernels (launchers return 0 or an error code)
 int ceb_gemm_launch(const ceb_wplane& w, const void* act_f16, int act_rows_capacity, const ceb_gemm_args& a,
                     cudaStream_t stream, int max_ctas = 0);
+// The dense product of a few rows with the extended epilogue (all of a's out_type, act, res and
+// strides are read; w has one group).
+bool ceb_linear_is_few(const ceb_wplane& w, int m);  // whether it is the quicker one for m rows
+int ceb_linear_few(const ceb_wplane& w, const void* x_f16, const ceb_gemm_args& a, cudaStream_t st);
 int ceb_repack_weights(ceb_wplane* dst, int ggml_type, const void* host_raw, int n_groups, int n_out, int k,
                        cudaStream_t stream);
 void ceb_wplane_free(ceb_wplane* w);

@@ -388,7 +388,7 @@ def _fused(lin, x, out_dtype, bias=None, act="none", residual=None, **kw):
 
 @pytest.mark.parametrize("wtype", [GGML_F16, GGML_Q8_0, GGML_Q4_K])
 @pytest.mark.parametrize("n,k", [(128, 256), (256, 256), (768, 768), (384, 512)])
-@pytest.mark.parametrize("m", [1, 2, 7, 33, 130, 300])
+@pytest.mark.parametrize("m", [1, 2, 7, 33, 130, 300, 1409])
 def test_linear_fused_sizes(cuda, wtype, n, k, m):
     g = torch.Generator().manual_seed(m)
     lin = _linear(cuda, wtype, n, k)
@@ -401,7 +401,7 @@ def test_linear_fused_sizes(cuda, wtype, n, k, m):
 @pytest.mark.parametrize("act", list(binding.ACTIVATIONS))
 @pytest.mark.parametrize("out_dtype", [HF, BF, FP])
 @pytest.mark.parametrize("res_dtype", [None, HF, BF, FP])
-@pytest.mark.parametrize("n,m", [(256, 3), (128, 45), (256, 300)])
+@pytest.mark.parametrize("n,m", [(256, 3), (128, 45), (256, 300), (256, 1301), (128, 2500)])
 def test_linear_fused_epilogues(cuda, act, out_dtype, res_dtype, n, m):
     g = torch.Generator().manual_seed(m)
     lin = _linear(cuda, GGML_F16, n, 128)
@@ -412,19 +412,25 @@ def test_linear_fused_epilogues(cuda, act, out_dtype, res_dtype, n, m):
         R.check(got, *want)
 
 
-def test_linear_fused_as_forward(cuda):
-    """Without residual and with the activations that ceb_linear_forward has: its bits."""
-    layer, _, _ = _linear(cuda, GGML_Q8_0, 256, 256)
-    x = torch.randn(300, 256, device=cuda).half()
+@pytest.mark.parametrize("m", [300, 3000])
+def test_linear_fused_beside_forward(cuda, m):
+    """Without residual and with the activations that ceb_linear_forward has: the same function, held to
+    the same bound (few rows run on another kernel, whose sums have another order); where both
+    run the tcgen05 kernel, the same bits."""
+    layer, w, rounded = _linear(cuda, GGML_Q8_0, 256, 256)
+    x = torch.randn(m, 256, device=cuda).half()
     bias = torch.randn(256, device=cuda)
     for gelu in (False, True):
         for dt in (HF, FP):
-            a = layer.fused(x, bias=bias, act="gelu" if gelu else "none", out_dtype=dt)
-            assert torch.equal(a, layer(x, bias=bias, gelu=gelu, out_f16=dt == HF))
+            act = "gelu" if gelu else "none"
+            a, b = layer.fused(x, bias=bias, act=act, out_dtype=dt), layer(x, bias=bias, gelu=gelu, out_f16=dt == HF)
+            for y in (a, b):
+                R.check(y, *R.linear(x, w, bias, act, None, dt, rounded))
+            assert m == 300 or torch.equal(a, b)
 
 
 @pytest.mark.parametrize("n", [128, 256])
-@pytest.mark.parametrize("m", [1, 5, 77, 300])
+@pytest.mark.parametrize("m", [1, 5, 77, 300, 2391])
 @pytest.mark.parametrize("dtype", [HF, FP])
 def test_linear_fused_strides_and_in_place(cuda, n, m, dtype):
     lin = _linear(cuda, GGML_F16, n, 192)
