@@ -21,6 +21,10 @@ struct Args {
     int* err;
 };
 
+// The kernels (attn_masked_f16.cu, attn_masked_bf16.cu).
+int launch_f16(const Args& a, cudaStream_t st);
+int launch_bf16(const Args& a, cudaStream_t st);
+
 // One sequence: query rows q0 .. q0+n-1, key rows k0 .. k0+m-1, the first `prefix` keys seen
 // by every row.
 struct Seq {

@@ -1,0 +1,6 @@
+// attn_masked_bf16.cu -- the masked attention kernels on bf16 values.
+#include "attn_tile.cuh"
+
+int ceb_am::launch_bf16(const Args& a, cudaStream_t st) {
+    return a.head_dim <= 64 ? by_kind<__nv_bfloat16, 64>(a, st) : by_kind<__nv_bfloat16, 128>(a, st);
+}

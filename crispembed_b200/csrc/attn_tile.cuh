@@ -1,0 +1,993 @@
+// attn_tile.cuh -- attention with shared key heads, score capping, a bias by distance and
+// masks, over packed sequences (ceb_attention_masked), on single-CTA tcgen05 MMAs.
+//
+// An item is (sequence, key head, query tile).  A tile's 128 MMA rows are query rows times
+// the query heads that share the key head (row r: query r / group, head r % group), so a
+// key tile is read once for all of them.  Keys stream in chunks; per chunk
+//   S = Q K^T   M = 128, N = the chunk's keys, fp32 in TMEM; head dims that are no multiple
+//               of 64 are filled up with zeros by the loads,
+//   softmax     one thread per row: score cap, bias, mask, the running maximum and sum in
+//               fp32, exponentials in fp32, weights rounded to the inputs' type (the MMA's
+//               operands have one type) into TMEM,
+//   O += P V    P from TMEM, V MN-major from shared memory, fp32 in TMEM.
+// The maximum that the exponentials use is raised -- and O rescaled -- only when the true one
+// exceeds it by 2^RAISE; fp16 weights carry a factor 2^UP so that small ones stay normal
+// numbers (both sums carry it, and the division drops it).
+//
+// A block goes on to items of blocks that have not started (cluster launch control), so
+// ragged items spread over the SMs without a counter in memory: calls hold no state.  The
+// loading warp runs ahead: it decodes items into a ring in shared memory, skips chunks that
+// no row of the tile sees (window, prefix, document ranges) and marks chunks that need a
+// mask.
+//
+// What hidden keys hold must not reach a sum.  Their scores are replaced before the softmax.
+// In P V, 0 times inf or NaN would be NaN: rows of a V tile past the sequence's end are
+// cleared, and a row whose result is not finite is computed again by one warp that reads
+// visible keys only (warp_row).
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <type_traits>
+
+#include "../../include/ceb_ops.h"
+#include "attn_masked.h"
+#include "ceb_internal.h"
+
+namespace {
+using namespace ceb_am;
+
+constexpr int QT = 128;   // rows of a tile (MMA M)
+constexpr int NTHR = 256; // warp 0 loads, warp 1 TMEM + MMA, warps 4..7 softmax
+constexpr int NRING = 4;  // items handed from the loading warp to the others
+
+template <int HD>
+struct Cfg {
+    static constexpr int KC = HD == 64 ? 96 : 64;           // keys a chunk
+    static constexpr int QB = HD == 64 ? 2 : 1;             // Q buffers
+    static constexpr int NS = HD == 64 ? 3 : 2;             // stages of K and of V
+    static constexpr int ND = NS + 2;                       // chunk descriptions
+    static constexpr int Q_BYTES = QT * HD * 2;             // 64-wide parts, one behind the other
+    static constexpr int K_BYTES = KC * HD * 2;             // K or V of a chunk
+    // two buffers of S, whose columns then hold P; O behind them
+    static constexpr uint32_t O_COL = 2 * KC, TMEM_COLS = 256;
+    static_assert(O_COL + HD <= TMEM_COLS, "TMEM plan");
+    enum { B_QFULL, B_QFREE = B_QFULL + 2, B_KFULL = B_QFREE + 2, B_KFREE = B_KFULL + NS, B_VFULL = B_KFREE + NS,
+           B_VFREE = B_VFULL + NS, B_CHUNK = B_VFREE + NS, B_SFULL = B_CHUNK + ND, B_PFULL = B_SFULL + 2,
+           B_PVDONE = B_PFULL + 2, B_DRAIN, B_NEXT, B_IFULL, B_IFREE = B_IFULL + NRING, NBAR = B_IFREE + NRING };
+};
+
+// A decoded item: query rows i0 .. of the tile (local), its sequence, key head; `empty`: no
+// key is seen by any row.  kvh < 0 ends the stream.
+struct Item {
+    Seq s;
+    int i0, kvh, empty;
+};
+struct alignas(16) Chunk {
+    int k0, flags, steps, pad;  // first key (local), 16-key steps that hold a key of the sequence
+};
+constexpr int MAX_BARS = 48, MAX_ND = 5;
+enum { LAST = 1, MASKED = 2, DOCS = 4 };
+
+struct Small {  // shared memory behind the tiles
+    uint64_t bars[MAX_BARS];
+    alignas(16) uint32_t answer[4];
+    uint32_t tmem;
+    int abort;
+    Item ring[NRING];
+    Chunk chunk[MAX_ND];
+    int docs[MAX_ND][96];
+    float2 ml[QT];  // (maximum, sum) of a row, for the join of a split item
+};
+// two warpgroups: their shares add up to the launch's 256 x 128 registers
+constexpr int CONTROL_REGS = 64, ROW_REGS = 192;
+static_assert(128 * (CONTROL_REGS + ROW_REGS) == NTHR * 128, "register shares");
+template <int N>
+CEB_DEV void regs_down() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+CEB_DEV void regs_up() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <int HD>
+constexpr size_t smem_bytes() {
+    return 1024 + Cfg<HD>::QB * Cfg<HD>::Q_BYTES + 2 * Cfg<HD>::NS * Cfg<HD>::K_BYTES + sizeof(Small);
+}
+static_assert(Cfg<64>::NBAR <= MAX_BARS && Cfg<128>::NBAR <= MAX_BARS && Cfg<64>::ND <= MAX_ND, "shared memory plan");
+static_assert(2 * (smem_bytes<64>() + 1024) <= 228 * 1024 && 2 * (smem_bytes<128>() + 1024) <= 228 * 1024,
+              "two blocks per SM");
+
+constexpr float LOG2E = 1.4426950408889634f;
+template <typename T>
+constexpr float RAISE = std::is_same<T, __half>::value ? 4.0f : 8.0f;
+template <typename T>
+constexpr float UP = std::is_same<T, __half>::value ? 8.0f : 0.0f;
+
+CEB_DEV float ex2f(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+CEB_DEV float rcpf(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+CEB_DEV float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+CEB_DEV uint32_t pack(float a, float b, __half) { return h2_as_u32(__floats2half2_rn(a, b)); }
+CEB_DEV uint32_t pack(float a, float b, __nv_bfloat16) {
+    __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&r);
+}
+// Whether a wait that began at clock t0 is over without its barrier: another role gave up, or
+// the time is up (about a second), which is recorded with the barrier's number.
+__device__ __noinline__ bool wait_over(volatile int* abort, int* err, uint32_t t0, int barrier) {
+    if (*abort) return true;
+    if ((uint32_t)clock() - t0 < (uint32_t)CEB_WAIT_LIMIT_CYCLES) return false;
+    *abort = 1;
+    if (err) atomicCAS(err, 0, (int)CEB_DEVERR_TIMEOUT_MMA | ((barrier + 1) << 16));
+    return true;
+}
+// MN-major operand, 128-byte swizzle: parts of 64 values along N `part` bytes apart, rows of
+// 128 B along K in groups of eight.
+CEB_DEV uint64_t v_desc(uint32_t saddr, uint32_t part) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+    d |= (uint64_t)(part >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+template <typename T>
+CEB_DEV uint32_t mma_desc(int n) {
+    return idesc_f16_f32(QT, n) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10));
+}
+// The bits of a 32-key piece that starts `at` keys into the row's frame: keys lo <= j < hi.
+CEB_DEV uint32_t span_bits(int lo, int hi, int at) {
+    const int a = min(max(lo - at, 0), 32), b = min(max(hi - at, 0), 32);
+    const uint32_t up = b >= 32 ? 0xffffffffu : (1u << b) - 1u, dn = a >= 32 ? 0xffffffffu : (1u << a) - 1u;
+    return up & ~dn;
+}
+
+// Products of 16 keys, the first of them d0 behind the row's place, into scores in log2 units.
+CEB_DEV void score_piece(const Args& a, uint32_t (&v)[16], int d0, float scale2, float slope2, const float* table) {
+    if (a.cap > 0.0f) {
+        const float in = 2.0f * scale2 / a.cap, up = a.cap * LOG2E;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {  // tanh y = 1 - 2 / (1 + e^2y)
+            const float e = ex2f(__uint_as_float(v[t]) * in);
+            v[t] = __float_as_uint(up * fmaf(-2.0f, rcpf(1.0f + e), 1.0f));
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < 16; ++t) v[t] = __float_as_uint(__uint_as_float(v[t]) * scale2);
+    }
+    if (a.slopes) {
+        const float d = (float)d0;
+#pragma unroll
+        for (int t = 0; t < 16; ++t)
+            v[t] = __float_as_uint(fmaf(slope2, fabsf(d + (float)t), __uint_as_float(v[t])));
+    }
+    if (table) {
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            const float b = __ldg(table + min(max(d0 + t, -a.radius), a.radius)), b2 = b * LOG2E;
+            // the lowest numbers stay numbers: -inf alone hides
+            v[t] = __float_as_uint(__uint_as_float(v[t]) + (b2 == -INFINITY && b != -INFINITY ? -3.402823466e38f : b2));
+        }
+    }
+}
+// The same on a row's registers, N products from key distance d0 on, one form each.
+// slopes: on one side of the diagonal the bias is linear in the key (side: keys before (-1) or
+// behind (1) the place of every row of the warp, 0 mixed).
+template <int N>
+CEB_DEV void scores_slopes(uint32_t (&v)[N], int d0, int side, float scale2, float slope2) {
+    if (side != 0) {
+        const float c = side < 0 ? -slope2 : slope2;
+        const f32x2 s2 = f2_splat(scale2), c2 = f2_splat(c), b2 = f2_splat(c * (float)d0);
+#pragma unroll
+        for (int t = 0; t < N; t += 2) {
+            float x, y;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(v[t]), __uint_as_float(v[t + 1])), s2,
+                             f2_fma(f2_pack((float)t, (float)(t + 1)), c2, b2)), x, y);
+            v[t] = __float_as_uint(x);
+            v[t + 1] = __float_as_uint(y);
+        }
+    } else {
+        const float d = (float)d0;
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+            v[t] = __float_as_uint(fmaf(__uint_as_float(v[t]), scale2, slope2 * fabsf(d + (float)t)));
+    }
+}
+// c tanh(s / c).  With every |s| of the warp's rows up to c, y P(y^2) with P fitted to tanh(y) / y
+// on [0, 1] for least relative error (2e-7 in fp32): multiply-adds alone.  Beyond,
+// 1 - 2 / (1 + e^2y), two special-function results a score.
+template <int N>
+CEB_DEV void scores_capped(uint32_t (&v)[N], float scale2, float cap2) {
+    const float in = scale2 / cap2;
+    float top = 0.0f;
+#pragma unroll
+    for (int t = 0; t < N; t += 2) top = max3(top, fabsf(__uint_as_float(v[t])), fabsf(__uint_as_float(v[t + 1])));
+    if (__all_sync(0xffffffffu, top * in <= 1.0f)) {
+        const f32x2 in2 = f2_splat(in), up2 = f2_splat(cap2);
+#pragma unroll
+        for (int t = 0; t < N; t += 2) {
+            const f32x2 y = f2_mul(f2_pack(__uint_as_float(v[t]), __uint_as_float(v[t + 1])), in2), z = f2_mul(y, y);
+            f32x2 p = f2_splat(0.0010410225950181484f);
+            p = f2_fma(p, z, f2_splat(-0.0062033794820308685f));
+            p = f2_fma(p, z, f2_splat(0.020289981737732887f));
+            p = f2_fma(p, z, f2_splat(-0.05345702916383743f));
+            p = f2_fma(p, z, f2_splat(0.13325203955173492f));
+            p = f2_fma(p, z, f2_splat(-0.33332839608192444f));
+            p = f2_fma(p, z, f2_splat(0.9999999403953552f));
+            float a, b;
+            f2_unpack(f2_mul(f2_mul(y, up2), p), a, b);
+            v[t] = __float_as_uint(a);
+            v[t + 1] = __float_as_uint(b);
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            const float e = ex2f(__uint_as_float(v[t]) * (2.0f * LOG2E * in));
+            v[t] = __float_as_uint(cap2 * fmaf(-2.0f, rcpf(1.0f + e), 1.0f));
+        }
+    }
+}
+// Bias by distance from the head's table.  False (v then holds nothing) if an entry times log2 e
+// passes the lowest number.
+template <int N>
+CEB_DEV bool scores_table(uint32_t (&v)[N], int d0, int radius, float scale2, const float* table) {
+    float low = 0.0f;
+    const bool far = d0 >= radius || d0 + N - 1 <= -radius, inner = d0 >= -radius && d0 + N - 1 <= radius;
+    if (__all_sync(0xffffffffu, far)) {
+        const float b = __ldg(table + (d0 > 0 ? radius : -radius)) * LOG2E;
+        low = b;
+        const f32x2 s2 = f2_splat(scale2), b2 = f2_splat(b);
+#pragma unroll
+        for (int t = 0; t < N; t += 2) {
+            float x, y;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(v[t]), __uint_as_float(v[t + 1])), s2, b2), x, y);
+            v[t] = __float_as_uint(x);
+            v[t + 1] = __float_as_uint(y);
+        }
+    } else if (__all_sync(0xffffffffu, inner)) {
+        const float* p = table + d0;
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            const float b = __ldg(p + t) * LOG2E;
+            low = fminf(low, b);
+            v[t] = __float_as_uint(fmaf(__uint_as_float(v[t]), scale2, b));
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            const float b = __ldg(table + min(max(d0 + t, -radius), radius)) * LOG2E;
+            low = fminf(low, b);
+            v[t] = __float_as_uint(fmaf(__uint_as_float(v[t]), scale2, b));
+        }
+    }
+    return !__any_sync(0xffffffffu, low == -INFINITY);
+}
+// The masks of a chunk's keys for one row: bit t of word c is key k0 + 32 c + t.
+struct Words {
+    uint32_t w[3];
+};
+template <int KC>
+__device__ __noinline__ Words seen_chunk(const Args& a, const Seq& s, int place, int k0, int doc, const int* docs) {
+    int lo, hi;
+    window(a, s, place, lo, hi);
+    Words r;
+#pragma unroll
+    for (int c = 0; c < KC / 32; ++c) {
+        const int at = k0 + 32 * c;
+        r.w[c] = (span_bits(lo, hi, at) | span_bits(0, s.prefix, at)) & span_bits(0, s.m, at);
+        if (docs) {
+            uint32_t same = 0;
+#pragma unroll 8
+            for (int t = 0; t < 32; ++t) same |= (uint32_t)(docs[32 * c + t] == doc) << t;
+            r.w[c] &= doc >= 0 ? same : 0u;
+        }
+    }
+    return r;
+}
+// Scores of a chunk, prepared in TMEM 16 at a time: any combination.
+template <int KC>
+__device__ __noinline__ void prepare_scores(const Args& a, uint32_t s_t, int d0, float scale2, float slope2, const float* table) {
+#pragma unroll 1
+    for (int c = 0; c < KC; c += 16) {
+        uint32_t v[16];
+        tmem_ld16(s_t + (uint32_t)c, v);
+        tmem_ld_wait();
+        score_piece(a, v, d0 + c, scale2, slope2, table);
+        tmem_st16(s_t + (uint32_t)c, v);
+    }
+    tmem_st_wait();
+}
+
+// SPLIT: the keys of an item are divided among the blocks of a cluster, which join their
+// sums through distributed shared memory; one item a block.
+// KIND: what stands between products and scores.  One of them is done in the registers that
+// hold a row's products (PLAIN: the scale, in the exponentials' multiply-add); combinations, and
+// scales that are not positive (the products' order is then not the scores'), take ANY, which
+// prepares the scores in TMEM first.
+enum { PLAIN, SLOPES, CAPPED, TABLE, ANY };
+
+template <typename T, int HD, int KIND, bool SPLIT>
+__global__ void __launch_bounds__(NTHR, 2)
+    attn_tile_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                     const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Args a, int n_tiles, int n_kv, int n_items,
+                     int batch, int parts) {
+    using C = Cfg<HD>;
+    constexpr int KC = C::KC, PC = KC / 32, NS = C::NS, ND = C::ND;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sQ = base;
+    uint8_t* sK = base + C::QB * C::Q_BYTES;
+    uint8_t* sV = sK + NS * C::K_BYTES;
+    Small& sm = *reinterpret_cast<Small*>(sV + NS * C::K_BYTES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tile_rows = QT / a.group;  // query rows of a tile
+    const int part = SPLIT ? (int)cluster_ctarank() : 0;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::NBAR; ++i)
+            mbar_init(smem_u32(&sm.bars[i]), (i == C::B_PFULL || i == C::B_PFULL + 1) ? 4 : (i >= C::B_IFREE ? 5 : 1));
+        fence_mbar_init();
+        sm.abort = 0;
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&qmap);
+        tma_prefetch_desc(&kmap);
+        tma_prefetch_desc(&vmap);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&sm.tmem), C::TMEM_COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+    volatile int* abort = &sm.abort;
+    auto bar = [&](int i) { return smem_u32(&sm.bars[i]); };
+    // Bounded waits; the error word names the barrier.  Short on purpose: the roles' code competes
+    // for the instruction cache.
+    auto wait_at = [&](int i, uint32_t par) {
+        uint32_t t0 = 0;
+        for (uint32_t n = 0; !mbar_try_wait(bar(i), par); ++n) {
+            if (n == 0) t0 = (uint32_t)clock();
+            if ((n & 255) == 255 && wait_over(abort, a.err, t0, i)) return false;
+        }
+        return true;
+    };
+    auto wait_warp = [&](int i, uint32_t par) { return __all_sync(0xffffffffu, wait_at(i, par)) != 0; };
+
+    // A softmax thread holds a row of S: the control warps leave it registers.
+    if (warp < 4) {
+        regs_down<CONTROL_REGS>();
+    }
+    if (warp == 0) {
+        // ------------------------------------------------ items, Q, and K / V of each chunk
+        int g = 0, n_it = 0, n_ask = 0, n_q = 0;  // chunks, items, questions, items with keys
+        bool ok = true;
+        auto publish = [&](const Item& it) {
+            const int r = n_it % NRING;
+            if (n_it >= NRING && !wait_warp(C::B_IFREE + r, ((n_it / NRING) - 1) & 1)) return false;
+            if (lane == 0) {
+                sm.ring[r] = it;
+                mbar_arrive(bar(C::B_IFULL + r));
+            }
+            __syncwarp();
+            ++n_it;
+            return true;
+        };
+        auto ask = [&] {
+            if (lane == 0) {
+                fence_proxy_async_smem();  // the last answer has been read
+                mbar_arrive_expect_tx(bar(C::B_NEXT), 16);
+                next_block_request(smem_u32(sm.answer), bar(C::B_NEXT));
+            }
+            __syncwarp();
+            ++n_ask;
+        };
+        // A block stands for `batch` items side by side: lane l decodes item l, all lanes keep the
+        // set of those that are queries of a sequence (tiles past a sequence's end cost nothing more).
+        Item mine;
+        unsigned todo;
+        auto decode = [&](int block) {
+            const int item = block * batch + lane;
+            bool live = lane < batch && item < n_items;
+            if (live) {
+                const int tile = item % n_tiles, rest = item / n_tiles, seq = rest / n_kv;
+                mine.kvh = rest - seq * n_kv;
+                mine.i0 = tile * tile_rows;
+                mine.empty = 1;
+                live = load_seq(a, seq, tile == 0 && mine.kvh == 0, mine.s) && mine.i0 < mine.s.n;
+            }
+            todo = __ballot_sync(0xffffffffu, live);
+        };
+        int block = SPLIT ? (int)(blockIdx.x / parts) : (int)blockIdx.x;
+        decode(block);
+        if constexpr (!SPLIT) ask();
+        while (ok) {
+            if (!todo) {
+                if (SPLIT) break;
+                if (!(ok = wait_warp(C::B_NEXT, (n_ask - 1) & 1))) break;
+                block = next_block_answer(smem_u32(sm.answer));
+                __syncwarp();
+                if (block < 0) break;
+                ask();
+                decode(block);
+                continue;
+            }
+            const int from = __ffs(todo) - 1;
+            todo &= todo - 1;
+            Item it;
+            it.kvh = __shfl_sync(0xffffffffu, mine.kvh, from);
+            it.i0 = __shfl_sync(0xffffffffu, mine.i0, from);
+            it.s.q0 = __shfl_sync(0xffffffffu, mine.s.q0, from);
+            it.s.n = __shfl_sync(0xffffffffu, mine.s.n, from);
+            it.s.k0 = __shfl_sync(0xffffffffu, mine.s.k0, from);
+            it.s.m = __shfl_sync(0xffffffffu, mine.s.m, from);
+            it.s.prefix = __shfl_sync(0xffffffffu, mine.s.prefix, from);
+            const Seq& s = it.s;
+            const int last = min(it.i0 + tile_rows, s.n) - 1, shift = s.m - s.n;
+            int lo0, hi0, lo1, hi1;  // windows of the first and the last row: both ends rise with the row
+            window(a, s, it.i0 + shift, lo0, hi0);
+            window(a, s, last + shift, lo1, hi1);
+            const int n1 = (s.prefix + KC - 1) / KC;  // chunks of the prefix, then those of the windows
+            const int c0 = max(n1, lo0 / KC);
+            const int total = n1 + (hi1 > lo0 ? max((hi1 + KC - 1) / KC - c0, 0) : 0);
+            const int t_end = SPLIT ? (int)((int64_t)total * (part + 1) / parts) : total;
+            int t = SPLIT ? (int)((int64_t)total * part / parts) : 0;
+            int dq0 = INT32_MAX, dq1 = -1;  // documents of the tile's rows
+            bool q_none = false;            // a row is of none
+            if (a.doc_q) {
+                for (int i = it.i0 + lane; i <= last; i += 32) {
+                    const int d = a.doc_q[s.q0 + i];
+                    if (d >= 0) dq0 = min(dq0, d), dq1 = max(dq1, d);
+                    else q_none = true;
+                }
+                q_none = __any_sync(0xffffffffu, q_none) != 0;
+                dq0 = __reduce_min_sync(0xffffffffu, dq0);
+                dq1 = __reduce_max_sync(0xffffffffu, dq1);
+            }
+            // positions t .. t_end - 1, those left out that hold no document of the tile; a chunk is
+            // loaded once it is known whether another follows
+            const int qb = n_q % C::QB;
+            int pend = -1, kd[KC / 32], kp[KC / 32];  // the chunk to load; documents of chunk t and of that one
+            bool one_doc = false, one_doc_p = false;  // all rows and keys (of the tile and chunk) are of one document
+            for (bool more = true; more; ++t) {
+                const int k0 = (t < n1 ? t : c0 + t - n1) * KC;
+                if (t >= t_end) {
+                    more = false;
+                } else if (a.doc_k) {
+                    int mn = INT32_MAX, mx = -1;
+#pragma unroll
+                    for (int x = 0; x < KC / 32; ++x) {
+                        const int j = k0 + 32 * x + lane;
+                        kd[x] = j < s.m ? max(a.doc_k[s.k0 + j], -1) : -1;
+                    }
+#pragma unroll
+                    for (int x = 0; x < KC / 32; ++x)
+                        if (kd[x] >= 0) mn = min(mn, kd[x]), mx = max(mx, kd[x]);
+                    mx = __reduce_max_sync(0xffffffffu, mx);
+                    mn = __reduce_min_sync(0xffffffffu, mn);
+                    if (mx < dq0 || mn > dq1) continue;
+                    one_doc = !q_none && dq0 == dq1 && mn == mx && mn == dq0;
+#pragma unroll
+                    for (int x = 0; x < KC / 32; ++x) one_doc = __all_sync(0xffffffffu, one_doc && kd[x] >= 0) != 0;
+                }
+                if (pend < 0) {  // the first chunk, or that there is none
+                    it.empty = !more;
+                    if (!(ok = publish(it))) break;
+                    if (!more) break;
+                    if (n_q >= C::QB && !(ok = wait_warp(C::B_QFREE + qb, ((n_q / C::QB) - 1) & 1))) break;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(bar(C::B_QFULL + qb), tile_rows * a.group * 128 * (HD / 64));
+#pragma unroll
+                        for (int x = 0; x < HD / 64; ++x)
+                            tma_load_3d(smem_u32(sQ + qb * C::Q_BYTES + x * QT * 128), &qmap, bar(C::B_QFULL + qb), 64 * x,
+                                        it.kvh * a.group, s.q0 + it.i0);
+                    }
+                    __syncwarp();
+                    ++n_q;
+                } else {
+                    const int st = g % NS, ds = g % ND, j0 = pend;
+                    if (g >= NS && !(ok = wait_warp(C::B_KFREE + st, ((g / NS) - 1) & 1))) break;
+                    // (the description's slot: its last chunk, g - NS - 2, was done with before S of chunk g - NS)
+                    if (a.doc_k) {
+#pragma unroll
+                        for (int x = 0; x < KC / 32; ++x) sm.docs[ds][32 * x + lane] = kp[x];
+                    }
+                    __syncwarp();
+                    if (lane == 0) {
+                        const bool open = j0 + KC <= s.m && (j0 + KC <= s.prefix || (j0 >= lo1 && j0 + KC <= hi0));
+                        sm.chunk[ds] = Chunk{j0, (more ? 0 : LAST) | (a.doc_k && !one_doc_p ? MASKED | DOCS : open ? 0 : MASKED),
+                                             min(KC / 16, (s.m - j0 + 15) / 16), 0};
+                        mbar_arrive(bar(C::B_CHUNK + ds));
+                        mbar_arrive_expect_tx(bar(C::B_KFULL + st), C::K_BYTES);
+#pragma unroll
+                        for (int x = 0; x < HD / 64; ++x)
+                            tma_load_3d(smem_u32(sK + st * C::K_BYTES + x * KC * 128), &kmap, bar(C::B_KFULL + st), 64 * x,
+                                        it.kvh, s.k0 + j0);
+                    }
+                    __syncwarp();
+                    ++g;
+                    if (g > NS && !(ok = wait_warp(C::B_VFREE + st, (((g - 1) / NS) - 1) & 1))) break;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(bar(C::B_VFULL + st), C::K_BYTES);
+#pragma unroll
+                        for (int x = 0; x < HD / 64; ++x)
+                            tma_load_3d(smem_u32(sV + st * C::K_BYTES + x * KC * 128), &vmap, bar(C::B_VFULL + st), 64 * x,
+                                        it.kvh, s.k0 + j0);
+                    }
+                    __syncwarp();
+                }
+                pend = k0;
+#pragma unroll
+                for (int x = 0; x < KC / 32; ++x) kp[x] = kd[x];
+                one_doc_p = one_doc;
+            }
+        }
+        if (ok) {
+            Item end = {};
+            end.kvh = -1;
+            publish(end);
+        }
+        // what is in flight lands before the block can exit
+        if (lane == 0) {
+            if (!ok && n_ask > 0) mbar_wait(bar(C::B_NEXT), (n_ask - 1) & 1, nullptr, nullptr, 0);
+            for (int k = n_q > C::QB ? n_q - C::QB : 0; k < n_q; ++k)
+                mbar_wait(bar(C::B_QFULL + k % C::QB), (k / C::QB) & 1, nullptr, nullptr, 0);
+            for (int c = g > NS ? g - NS : 0; c < g; ++c) {
+                mbar_wait(bar(C::B_KFULL + c % NS), (c / NS) & 1, nullptr, nullptr, 0);
+                if (ok || c < g - 1) mbar_wait(bar(C::B_VFULL + c % NS), (c / NS) & 1, nullptr, nullptr, 0);
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------ MMA: S and P V, each as soon as it can be
+        // All lanes run along, one issues.
+        const bool one = elect_one();
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const int n16 = (a.head_dim + 15) / 16;
+        const uint32_t s_desc = mma_desc<T>(KC);
+        const uint32_t o_desc = mma_desc<T>(16 * n16) | (1u << 16);  // B (V) MN-major
+        int gs = 0, gp = 0, n_it = 0, n_q = 0;  // next S, next P V, items, items with keys
+        bool end = false, have = false, need_q = false, first = false;
+        uint32_t firsts = 0;      // bit g & 3: chunk g begins an item (its P V overwrites O)
+        int steps_of[2] = {0, 0};  // 16-key steps of the chunks whose P V is to come
+        auto test = [&](int i, uint32_t par) { return __all_sync(0xffffffffu, mbar_test(bar(i), par)) != 0; };
+        uint32_t t0 = 0;
+        for (uint32_t idle = 0;; ++idle) {
+            if (!end && !have && test(C::B_IFULL + n_it % NRING, (n_it / NRING) & 1)) {
+                const volatile Item& it = sm.ring[n_it % NRING];
+                const int kvh = __shfl_sync(0xffffffffu, it.kvh, 0), empty = __shfl_sync(0xffffffffu, it.empty, 0);
+                if (one) mbar_arrive(bar(C::B_IFREE + n_it % NRING));
+                ++n_it;
+                end = kvh < 0;
+                have = need_q = first = !end && !empty;
+                idle = 0;
+            }
+            if (have && gs - gp < 2 && (!need_q || test(C::B_QFULL + n_q % C::QB, (n_q / C::QB) & 1)) &&
+                test(C::B_KFULL + gs % NS, (gs / NS) & 1) &&
+                // S buffer gs & 1: the P V that reads chunk gs - 2's weights there is done (the last one
+                // issued is that one or a later one)
+                (gs < 2 || test(C::B_PVDONE, (gp - 1) & 1))) {
+                need_q = false;
+                const int st = gs % NS, qb = n_q % C::QB;
+                const volatile Chunk& ck = sm.chunk[gs % ND];
+                const bool last = (__shfl_sync(0xffffffffu, ck.flags, 0) & LAST) != 0;
+                const int steps = __shfl_sync(0xffffffffu, ck.steps, 0);
+                tc_fence_after();
+                const uint32_t qs = smem_u32(sQ) + qb * C::Q_BYTES, ks = smem_u32(sK) + st * C::K_BYTES;
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; ++kk)  // 16 values of the head: 32 B of a 64-wide part
+                    mma_f16_ss_if(one && kk < n16, tm + (uint32_t)((gs & 1) * KC),
+                                  smem_desc_sw128(qs + (kk >> 2) * QT * 128) + (uint64_t)(2 * (kk & 3)),
+                                  smem_desc_sw128(ks + (kk >> 2) * KC * 128) + (uint64_t)(2 * (kk & 3)), s_desc, kk != 0);
+                if (one) {
+                    mma_commit(bar(C::B_SFULL + (gs & 1)));
+                    mma_commit(bar(C::B_KFREE + st));
+                    if (last) mma_commit(bar(C::B_QFREE + qb));
+                }
+                if (gs & 1) steps_of[1] = steps;
+                else steps_of[0] = steps;
+                firsts = (firsts & ~(1u << (gs & 3))) | (uint32_t)first << (gs & 3);
+                first = false;
+                ++gs;
+                if (last) {
+                    have = false;
+                    ++n_q;
+                }
+                idle = 0;
+            }
+            if (gp < gs && test(C::B_PFULL + (gp & 1), (gp >> 1) & 1) && test(C::B_VFULL + gp % NS, (gp / NS) & 1)) {
+                const int st = gp % NS, steps = gp & 1 ? steps_of[1] : steps_of[0];
+                tc_fence_after();
+                const uint64_t vd = v_desc(smem_u32(sV) + st * C::K_BYTES, KC * 128);
+                const bool over = firsts >> (gp & 3) & 1u;
+#pragma unroll
+                for (int j = 0; j < KC / 16; ++j)  // 16 keys: 2048 B of V, 8 columns of P
+                    mma_f16_ts_if(one && j < steps, tm + C::O_COL, tm + (uint32_t)((gp & 1) * KC + 8 * j),
+                                  vd + (uint64_t)(128 * j), o_desc, !(over && j == 0));
+                if (one) {
+                    mma_commit(bar(C::B_PVDONE));
+                    mma_commit(bar(C::B_VFREE + st));
+                }
+                ++gp;
+                idle = 0;
+            }
+            if (end && gp == gs) break;
+            if (idle == 0) t0 = (uint32_t)clock();
+            if ((idle & 255) == 255) {  // bounded, as every wait
+                if (__any_sync(0xffffffffu, wait_over(abort, a.err, t0, C::B_DRAIN))) break;
+            }
+        }
+        if (one) mma_commit(bar(C::B_DRAIN));  // every MMA issued has finished before TMEM is freed
+        mbar_wait(bar(C::B_DRAIN), 0, nullptr, nullptr, 0);
+        __syncwarp();
+    } else if (warp >= 4) {
+        // ------------------------------------------------ softmax and output, thread = row
+        regs_up<ROW_REGS>();
+        const int qd = warp & 3;  // TMEM lanes 32 qd ..
+        const int row = 32 * qd + lane;
+        const uint32_t row_t = tmem + ((uint32_t)(32 * qd) << 16);
+        const int qi = row / a.group, head_in = row - qi * a.group;
+        const float scale2 = a.scale * LOG2E;
+        // scores in log2 units are (products or prepared scores) * mul
+        const float mul = KIND == PLAIN ? scale2 : 1.0f;
+        int g = 0;
+        bool ok = true;
+        // V rows past the sequence's end hold other rows of the buffer: cleared
+        auto clear_v = [&](int k0, int m) {
+            if (k0 + KC <= m) return true;
+            const int st = g % NS;
+            if (!wait_warp(C::B_VFULL + st, (g / NS) & 1)) return false;
+            if (row < KC && k0 + row >= m) {
+#pragma unroll
+                for (int x = 0; x < HD / 64; ++x)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        *reinterpret_cast<uint4*>(sV + st * C::K_BYTES + (x * KC + row) * 128 + 16 * c) =
+                            make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+            }
+            return true;
+        };
+        for (int n_it = 0; ok; ++n_it) {
+            const int r = n_it % NRING;
+            if (!(ok = wait_warp(C::B_IFULL + r, (n_it / NRING) & 1))) break;
+            // the item stays in the ring (released at its end): few of its numbers are worth a register
+            const Item& it = sm.ring[r];
+            if (it.kvh < 0) break;
+            const Seq& s = it.s;
+            const bool live = qi < tile_rows && it.i0 + qi < s.n;
+            const int place = it.i0 + qi + s.m - s.n;
+            const int doc = live && a.doc_q ? a.doc_q[s.q0 + it.i0 + qi] : 0;
+            float slope2 = 0.0f;
+            const float* table = nullptr;  // bias at distance 0
+            if (KIND != PLAIN && live) {
+                const int head = it.kvh * a.group + head_in;
+                if (a.slopes) slope2 = -a.slopes[head] * LOG2E;
+                if (a.table) table = a.table + (int64_t)head * (2 * (int64_t)a.radius + 1) + a.radius;
+            }
+            if (KIND >= TABLE && a.table && !table) table = a.table + a.radius;  // (a row that is none)
+            const bool empty = it.empty;
+            if (!__any_sync(0xffffffffu, live)) {
+                // none of the warp's rows is one: it keeps to the barriers and its share of V
+                for (bool last = empty; !last; ++g) {
+                    const int ds = g % ND;
+                    if (!(ok = wait_warp(C::B_CHUNK + ds, (g / ND) & 1) &&
+                               wait_warp(C::B_SFULL + (g & 1), (g >> 1) & 1)))
+                        break;
+                    const int k0 = sm.chunk[ds].k0;
+                    last = (sm.chunk[ds].flags & LAST) != 0;
+                    if (!(ok = clear_v(k0, s.m))) break;
+                    __syncwarp();
+                    // (as the others: a phase of P V is waited for before the next may complete)
+                    if (g > 0 && !(ok = wait_warp(C::B_PVDONE, (g - 1) & 1))) break;
+                    if (lane == 0) mbar_arrive(bar(C::B_PFULL + (g & 1)));
+                    __syncwarp();
+                }
+                if (!ok) break;
+                if constexpr (SPLIT) sm.ml[row] = make_float2(-INFINITY, 0.0f);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(C::B_IFREE + r));
+                continue;
+            }
+            float m_run = -INFINITY, l_run = 0.0f;  // the maximum in use (log2 units) and the sum
+            for (bool first = true; !empty; first = false) {
+                const int ds = g % ND;
+                if (!(ok = wait_warp(C::B_CHUNK + ds, (g / ND) & 1) &&
+                           wait_warp(C::B_SFULL + (g & 1), (g >> 1) & 1)))
+                    break;
+                tc_fence_after();
+                const Chunk ck = sm.chunk[ds];
+                const int k0 = ck.k0, flags = ck.flags;
+                const uint32_t s_t = row_t + (uint32_t)((g & 1) * KC);
+                if (!(ok = clear_v(k0, s.m))) break;
+                Words seen;
+                if (flags & MASKED) seen = seen_chunk<KC>(a, s, place, k0, doc, flags & DOCS ? sm.docs[ds] : nullptr);
+                const int d0 = k0 - place;
+                if constexpr (KIND == ANY) prepare_scores<KC>(a, s_t, d0, scale2, slope2, table);
+                uint32_t v[KC];
+                auto load = [&] {
+#pragma unroll
+                    for (int pc = 0; pc < PC; ++pc)
+                        tmem_ld32(s_t + (uint32_t)(32 * pc), reinterpret_cast<uint32_t(&)[32]>(v[32 * pc]));
+                    tmem_ld_wait();
+                };
+                load();
+                if constexpr (KIND == SLOPES) {
+                    const int side = __all_sync(0xffffffffu, d0 >= 0) ? 1 : __all_sync(0xffffffffu, d0 + KC - 1 <= 0) ? -1 : 0;
+                    scores_slopes(v, d0, side, scale2, slope2);
+                }
+                if constexpr (KIND == CAPPED) scores_capped(v, scale2, a.cap * LOG2E);
+                if constexpr (KIND == TABLE)
+                    if (!scores_table(v, d0, a.radius, scale2, table)) {
+                        prepare_scores<KC>(a, s_t, d0, scale2, slope2, table);
+                        load();
+                    }
+                if (flags & MASKED) {
+#pragma unroll
+                    for (int t = 0; t < KC; ++t)
+                        if (!(seen.w[t / 32] >> (t % 32) & 1u)) v[t] = 0xff800000u;  // -inf
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int t = 0; t < KC; t += 2)
+                    mx[(t >> 1) & 3] = max3(mx[(t >> 1) & 3], __uint_as_float(v[t]), __uint_as_float(v[t + 1]));
+                float cm = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
+                if (KIND == PLAIN) cm = cm == -INFINITY ? cm : cm * mul;  // (mul > 0)
+                const bool raise = __any_sync(0xffffffffu, cm > m_run + RAISE<T>) || first;
+                float alpha = 1.0f;
+                if (raise) {
+                    const float m_new = fmaxf(m_run, cm);
+                    alpha = m_new == -INFINITY ? 1.0f : ex2f(m_run - m_new);
+                    m_run = m_new;
+                }
+                const f32x2 nm2 = f2_splat(UP<T> - (m_run == -INFINITY ? 0.0f : m_run)), mul2 = f2_splat(mul);
+                f32x2 sum[2] = {f2_splat(0.0f), f2_splat(0.0f)};
+#pragma unroll
+                for (int pc = 0; pc < PC; ++pc) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int t = 0; t < 32; t += 2) {
+                        float e0, e1;
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(v[32 * pc + t]), __uint_as_float(v[32 * pc + t + 1])), mul2, nm2),
+                                  e0, e1);
+                        e0 = ex2f(e0);
+                        e1 = ex2f(e1);
+                        sum[(t >> 1) & 1] = f2_add(sum[(t >> 1) & 1], f2_pack(e0, e1));
+                        pk[t >> 1] = pack(e0, e1, T());
+                    }
+                    // the weights take the columns of scores that have been read
+                    tmem_st16(s_t + (uint32_t)(16 * pc), pk);
+                }
+                {
+                    float s0, s1;
+                    f2_unpack(f2_add(sum[0], sum[1]), s0, s1);
+                    l_run = l_run * alpha + (s0 + s1);
+                }
+                if (g > 0) {
+                    // P V of chunk g - 1 has added to O (waited for in every chunk: no phase is left out)
+                    if (!(ok = wait_warp(C::B_PVDONE, (g - 1) & 1))) break;
+                    tc_fence_after();
+                    if (raise && !first) {
+#pragma unroll 1
+                        for (int o0 = 0; o0 < HD; o0 += 32) {
+                            uint32_t ov[32];
+                            tmem_ld32(row_t + C::O_COL + (uint32_t)o0, ov);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int t = 0; t < 32; ++t) ov[t] = __float_as_uint(__uint_as_float(ov[t]) * alpha);
+                            tmem_st32(row_t + C::O_COL + (uint32_t)o0, ov);
+                        }
+                    }
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(C::B_PFULL + (g & 1)));
+                ++g;
+                if (flags & LAST) break;
+            }
+            // the item's last P V has finished: O / sum
+            ok = ok && (empty || wait_warp(C::B_PVDONE, (g - 1) & 1));
+            if (!ok) break;
+            tc_fence_after();
+            if constexpr (SPLIT) {
+                // this part's row, for the join: tiles of finished chunks make room for it
+                float* o = reinterpret_cast<float*>(sK) + row * HD;
+                sm.ml[row] = make_float2(m_run, l_run);
+                if (!empty) {
+#pragma unroll 1
+                    for (int o0 = 0; o0 < HD; o0 += 32) {
+                        uint32_t ov[32];
+                        tmem_ld32(row_t + C::O_COL + (uint32_t)o0, ov);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int t = 0; t < 32; t += 4)
+                            *reinterpret_cast<uint4*>(o + o0 + t) = make_uint4(ov[t], ov[t + 1], ov[t + 2], ov[t + 3]);
+                    }
+                }
+            } else {
+                const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+                bool wrong = l_run != l_run || l_run == INFINITY;
+                const int i = it.i0 + qi, head = it.kvh * a.group + head_in;
+                T* out = static_cast<T*>(a.out) + (int64_t)(s.q0 + i) * a.o_row + head * a.o_head;
+#pragma unroll 1
+                for (int o0 = 0; o0 < a.head_dim; o0 += 32) {
+                    uint32_t ov[32];
+                    if (!empty) {
+                        tmem_ld32(row_t + C::O_COL + (uint32_t)o0, ov);
+                        tmem_ld_wait();
+                    }
+#pragma unroll
+                    for (int t = 0; t < 32; t += 8) {
+                        if (o0 + t < a.head_dim) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                float x = __uint_as_float(ov[t + 2 * c]), y = __uint_as_float(ov[t + 2 * c + 1]);
+                                if (empty) x = y = 0.0f;
+                                wrong |= !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
+                                w[c] = pack(x * inv, y * inv, T());
+                            }
+                            if (live) *reinterpret_cast<uint4*>(out + o0 + t) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                }
+                // rows that met inf or NaN, be it their own or a hidden key's
+                for (unsigned b = __ballot_sync(0xffffffffu, live && wrong); b; b &= b - 1) {
+                    const int l = __ffs(b) - 1;
+                    __syncwarp();
+                    warp_row<T>(a, s, __shfl_sync(0xffffffffu, i, l), __shfl_sync(0xffffffffu, head, l));
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(C::B_IFREE + r));
+        }
+        if constexpr (SPLIT) {
+            // Each block joins every parts-th row, a warp a row, a lane four values of the head.
+            __syncwarp();
+            cluster_sync();
+            const int item = blockIdx.x / parts, tile = item % n_tiles, rest = item / n_tiles;
+            const int seq = rest / n_kv, kvh = rest - seq * n_kv, i0 = tile * tile_rows;
+            Seq s;
+            if (load_seq(a, seq, false, s) && i0 < s.n) {
+                const int rows = min(tile_rows, s.n - i0) * a.group;
+                const uint32_t ml = smem_u32(sm.ml), o = smem_u32(sK);
+                for (int r = part + parts * (warp - 4); r < rows; r += parts * 4) {
+                    float top = -INFINITY;
+                    for (int c = 0; c < parts; ++c) {
+                        float m;
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(m) : "r"(mapa_shared(ml + 8 * r, c)) : "memory");
+                        top = fmaxf(top, m);
+                    }
+                    float sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int c = 0; c < parts; ++c) {
+                        float m, l;
+                        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                                     : "=f"(m), "=f"(l)
+                                     : "r"(mapa_shared(ml + 8 * r, c))
+                                     : "memory");
+                        // a part without keys has no sums (its tiles hold anything)
+                        if (l == 0.0f && m == -INFINITY) continue;
+                        const float w = top == -INFINITY ? 1.0f : ex2f(m - top);
+                        sum += w * l;
+                        if (4 * lane < HD) {
+                            float x[4];
+                            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                         : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
+                                         : "r"(mapa_shared(o + (r * HD + 4 * lane) * 4, c))
+                                         : "memory");
+    #pragma unroll
+                            for (int k = 0; k < 4; ++k) acc[k] += w * x[k];
+                        }
+                    }
+                    const int i = i0 + r / a.group, head = kvh * a.group + r % a.group;
+                    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+                    bool wrong = sum != sum || sum == INFINITY;
+                    if (4 * lane < a.head_dim) {
+    #pragma unroll
+                        for (int k = 0; k < 4; ++k) wrong |= !(fabsf(acc[k]) < INFINITY);
+                        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(s.q0 + i) * a.o_row + head * a.o_head +
+                                                  4 * lane) =
+                            make_uint2(pack(acc[0] * inv, acc[1] * inv, T()), pack(acc[2] * inv, acc[3] * inv, T()));
+                    }
+                    if (__any_sync(0xffffffffu, wrong)) {
+                        __syncwarp();
+                        warp_row<T>(a, s, i, head);
+                    }
+                }
+            }
+        }
+    }
+
+    if constexpr (SPLIT) {
+        __syncwarp();
+        if (warp < 4) cluster_sync();
+        cluster_sync();  // no block of the cluster still reads this one's shared memory
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C::TMEM_COLS);
+    }
+}
+
+template <typename T, int HD, int KIND>
+int launch_tiles(const Args& a, cudaStream_t st) {
+    using C = Cfg<HD>;
+    constexpr bool bf16 = !std::is_same<T, __half>::value;
+    const int n_kv = a.n_head / a.group, tile_rows = QT / a.group;
+    const int n_tiles = (a.max_q + tile_rows - 1) / tile_rows;
+    const int64_t items = (int64_t)n_tiles * n_kv * a.n_seqs;
+    if (items > INT32_MAX / 8) return ceb_set_error(2, "attention_masked: %lld query tiles", (long long)items);
+    CUtensorMap qmap, kmap, vmap;
+    if (int rc = ceb_make_tmap_heads(&qmap, a.q, bf16, a.head_dim, a.n_head, a.q_rows, a.q_head, a.q_row, a.group, tile_rows))
+        return rc;
+    // (without key rows there is nothing to load: any map will do)
+    const bool keys = a.k_rows > 0;
+    if (int rc = ceb_make_tmap_heads(&kmap, keys ? a.k : a.q, bf16, a.head_dim, keys ? n_kv : a.n_head,
+                                     keys ? a.k_rows : a.q_rows, keys ? a.k_head : a.q_head, keys ? a.k_row : a.q_row, 1,
+                                     C::KC))
+        return rc;
+    if (int rc = ceb_make_tmap_heads(&vmap, keys ? a.v : a.q, bf16, a.head_dim, keys ? n_kv : a.n_head,
+                                     keys ? a.k_rows : a.q_rows, keys ? a.v_head : a.q_head, keys ? a.v_row : a.q_row, 1,
+                                     C::KC))
+        return rc;
+    // Few items with many keys: the keys of each are divided among a cluster, as long as that
+    // fills the SMs and leaves each part some chunks.
+    const int chunks = (a.max_k + C::KC - 1) / C::KC;
+    int parts = 1;
+    while (parts < 8 && items * parts * 2 <= 4 * ceb_num_sms() && chunks >= 4 * parts) parts *= 2;
+    const size_t smem = smem_bytes<HD>();
+    cudaLaunchConfig_t cfg = {};
+    // several items to a block where there are many: an item that is no query of its sequence
+    // (ragged batches have a third of those) then costs a lane's look, not a block
+    const int batch = parts > 1 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(32, items / (16 * ceb_num_sms())));
+    cfg.gridDim = dim3((unsigned)((items + batch - 1) / batch * parts));
+    cfg.blockDim = dim3(NTHR);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = parts;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    // (split items, few rows each, are bound by their keys' bytes: two kinds will do)
+    auto kernel = parts > 1 ? attn_tile_kernel<T, HD, KIND == PLAIN ? PLAIN : ANY, true> : attn_tile_kernel<T, HD, KIND, false>;
+    if (int rc = ceb_func_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
+    cudaError_t e = cudaSuccess;
+    CEB_LAUNCH(CEB_PROF_ATTN, st, 0.0, 0.0,
+               e = cudaLaunchKernelEx(&cfg, kernel, qmap, kmap, vmap, a, n_tiles, n_kv, (int)items, batch, parts));
+    CEB_CUDA_OK(e);
+    return 0;
+}
+
+template <typename T, int HD>
+int by_kind(const Args& a, cudaStream_t st) {
+    if (!(a.scale > 0.0f) || (a.cap > 0.0f && (a.slopes || a.table))) return launch_tiles<T, HD, ANY>(a, st);
+    if (a.cap > 0.0f) return launch_tiles<T, HD, CAPPED>(a, st);
+    if (a.slopes) return launch_tiles<T, HD, SLOPES>(a, st);
+    if (a.table) return launch_tiles<T, HD, TABLE>(a, st);
+    return launch_tiles<T, HD, PLAIN>(a, st);
+}
+
+}  // namespace
