@@ -56,8 +56,8 @@ struct Cfg {
     static constexpr uint32_t O_COL = 2 * KC, TMEM_COLS = 256;
     static_assert(O_COL + HD <= TMEM_COLS, "TMEM plan");
     enum { B_QFULL, B_QFREE = B_QFULL + 2, B_KFULL = B_QFREE + 2, B_KFREE = B_KFULL + NS, B_VFULL = B_KFREE + NS,
-           B_VFREE = B_VFULL + NS, B_CHUNK = B_VFREE + NS, B_SFULL = B_CHUNK + ND, B_PFULL = B_SFULL + 2,
-           B_PVDONE = B_PFULL + 2, B_DRAIN, B_NEXT, B_IFULL, B_IFREE = B_IFULL + NRING, NBAR = B_IFREE + NRING };
+           B_VFREE = B_VFULL + NS, B_SFULL = B_VFREE + NS, B_PFULL = B_SFULL + 2,
+           B_PVDONE = B_PFULL + 2, B_DRAIN = B_PVDONE + 2, B_NEXT, B_IFULL, B_IFREE = B_IFULL + NRING, NBAR = B_IFREE + NRING };
 };
 
 // A decoded item: query rows i0 .. of the tile (local), its sequence, key head; `empty`: no
@@ -67,10 +67,10 @@ struct Item {
     int i0, kvh, empty;
 };
 struct alignas(16) Chunk {
-    int k0, flags, steps, pad;  // first key (local), 16-key steps that hold a key of the sequence
+    int k0, flags, steps, docs;  // first key (local), 16-key steps that hold a key, slot of the documents
 };
 constexpr int MAX_BARS = 48, MAX_ND = 5;
-enum { LAST = 1, MASKED = 2, DOCS = 4 };
+enum { LAST = 1, MASKED = 2, DOCS = 4, TAIL = 8 };  // TAIL: the sequence ends in it
 
 struct Small {  // shared memory behind the tiles
     uint64_t bars[MAX_BARS];
@@ -78,7 +78,8 @@ struct Small {  // shared memory behind the tiles
     uint32_t tmem;
     int abort;
     Item ring[NRING];
-    Chunk chunk[MAX_ND];
+    Chunk chunk[MAX_ND];  // from the loading warp to the MMA warp
+    Chunk now[2];         // of the S buffers, from there to the softmax
     int docs[MAX_ND][96];
     float2 ml[QT];  // (maximum, sum) of a row, for the join of a split item
 };
@@ -342,9 +343,10 @@ __global__ void __launch_bounds__(NTHR, 2)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::NBAR; ++i)
-            mbar_init(smem_u32(&sm.bars[i]), (i == C::B_PFULL || i == C::B_PFULL + 1) ? 4 : (i >= C::B_IFREE ? 5 : 1));
+            mbar_init(smem_u32(&sm.bars[i]), (i == C::B_PFULL || i == C::B_PFULL + 1) ? 4 : (i == C::B_SFULL || i == C::B_SFULL + 1) ? 2 : (i >= C::B_IFREE ? 5 : 1));
         fence_mbar_init();
         sm.abort = 0;
+        sm.now[0] = sm.now[1] = Chunk{0, 0, 0, 0};
     }
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&qmap);
@@ -361,8 +363,7 @@ __global__ void __launch_bounds__(NTHR, 2)
     const uint32_t tmem = sm.tmem;
     volatile int* abort = &sm.abort;
     auto bar = [&](int i) { return smem_u32(&sm.bars[i]); };
-    // Bounded waits; the error word names the barrier.  Short on purpose: the roles' code competes
-    // for the instruction cache.
+    // Bounded waits; the error word names the barrier.  Most barriers are through when they are asked.
     auto wait_at = [&](int i, uint32_t par) {
         uint32_t t0 = 0;
         for (uint32_t n = 0; !mbar_try_wait(bar(i), par); ++n) {
@@ -514,9 +515,9 @@ __global__ void __launch_bounds__(NTHR, 2)
                     __syncwarp();
                     if (lane == 0) {
                         const bool open = j0 + KC <= s.m && (j0 + KC <= s.prefix || (j0 >= lo1 && j0 + KC <= hi0));
-                        sm.chunk[ds] = Chunk{j0, (more ? 0 : LAST) | (a.doc_k && !one_doc_p ? MASKED | DOCS : open ? 0 : MASKED),
-                                             min(KC / 16, (s.m - j0 + 15) / 16), 0};
-                        mbar_arrive(bar(C::B_CHUNK + ds));
+                        sm.chunk[ds] = Chunk{j0, (more ? 0 : LAST) | (j0 + KC > s.m ? TAIL : 0) |
+                                                 (a.doc_k && !one_doc_p ? MASKED | DOCS : open ? 0 : MASKED),
+                                             min(KC / 16, (s.m - j0 + 15) / 16), ds};
                         mbar_arrive_expect_tx(bar(C::B_KFULL + st), C::K_BYTES);
 #pragma unroll
                         for (int x = 0; x < HD / 64; ++x)
@@ -569,71 +570,91 @@ __global__ void __launch_bounds__(NTHR, 2)
         uint32_t firsts = 0;      // bit g & 3: chunk g begins an item (its P V overwrites O)
         int steps_of[2] = {0, 0};  // 16-key steps of the chunks whose P V is to come
         auto test = [&](int i, uint32_t par) { return __all_sync(0xffffffffu, mbar_test(bar(i), par)) != 0; };
+        auto issue_s = [&] {
+            const int st = gs % NS, qb = n_q % C::QB;
+            const Chunk ck = sm.chunk[gs % ND];
+            const bool last = (__shfl_sync(0xffffffffu, ck.flags, 0) & LAST) != 0;
+            tc_fence_after();
+            const uint32_t qs = smem_u32(sQ) + qb * C::Q_BYTES, ks = smem_u32(sK) + st * C::K_BYTES;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk)  // 16 values of the head: 32 B of a 64-wide part
+                mma_f16_ss_if(one && kk < n16, tm + (uint32_t)((gs & 1) * KC),
+                              smem_desc_sw128(qs + (kk >> 2) * QT * 128) + (uint64_t)(2 * (kk & 3)),
+                              smem_desc_sw128(ks + (kk >> 2) * KC * 128) + (uint64_t)(2 * (kk & 3)), s_desc, kk != 0);
+            if (one) {
+                mma_commit(bar(C::B_SFULL + (gs & 1)));
+                mma_commit(bar(C::B_KFREE + st));
+                if (last) mma_commit(bar(C::B_QFREE + qb));
+                sm.now[gs & 1] = ck;
+                mbar_arrive(bar(C::B_SFULL + (gs & 1)));
+            }
+            const int steps = __shfl_sync(0xffffffffu, ck.steps, 0);
+            if (gs & 1) steps_of[1] = steps;
+            else steps_of[0] = steps;
+            firsts = (firsts & ~(1u << (gs & 3))) | (uint32_t)first << (gs & 3);
+            first = false;
+            ++gs;
+            if (last) {
+                have = false;
+                ++n_q;
+            }
+        };
+        auto issue_pv = [&] {
+            const int st = gp % NS, steps = gp & 1 ? steps_of[1] : steps_of[0];
+            tc_fence_after();
+            const uint64_t vd = v_desc(smem_u32(sV) + st * C::K_BYTES, KC * 128);
+            const bool over = firsts >> (gp & 3) & 1u;
+#pragma unroll
+            for (int j = 0; j < KC / 16; ++j)  // 16 keys: 2048 B of V, 8 columns of P
+                mma_f16_ts_if(one && j < steps, tm + C::O_COL, tm + (uint32_t)((gp & 1) * KC + 8 * j),
+                              vd + (uint64_t)(128 * j), o_desc, !(over && j == 0));
+            if (one) {
+                mma_commit(bar(C::B_PVDONE + (gp & 1)));
+                mma_commit(bar(C::B_VFREE + st));
+            }
+            ++gp;
+        };
+        // S runs up to two chunks ahead of P V.  Of what a turn waits for, what comes first is asked first:
+        // after P V of chunk g its end, which leaves S buffer g & 1 to chunk g + 2, then that chunk's K or
+        // the weights of chunk g + 1, whichever is there.
+        bool ok = true;
         uint32_t t0 = 0;
-        for (uint32_t idle = 0;; ++idle) {
-            if (!end && !have && test(C::B_IFULL + n_it % NRING, (n_it / NRING) & 1)) {
+        for (uint32_t idle = 0; ok; ++idle) {
+            if (gs - gp == 2 || (end && gp < gs)) {
+                if (!(ok = wait_warp(C::B_PFULL + (gp & 1), (gp >> 1) & 1) && wait_warp(C::B_VFULL + gp % NS, (gp / NS) & 1))) break;
+                issue_pv();
+                if (!end && !(ok = wait_warp(C::B_PVDONE + ((gp - 1) & 1), ((gp - 1) >> 1) & 1))) break;
+                idle = 0;
+                continue;
+            }
+            if (end) break;
+            if (!have && test(C::B_IFULL + n_it % NRING, (n_it / NRING) & 1)) {
                 const volatile Item& it = sm.ring[n_it % NRING];
                 const int kvh = __shfl_sync(0xffffffffu, it.kvh, 0), empty = __shfl_sync(0xffffffffu, it.empty, 0);
+                __syncwarp();
                 if (one) mbar_arrive(bar(C::B_IFREE + n_it % NRING));
                 ++n_it;
                 end = kvh < 0;
                 have = need_q = first = !end && !empty;
                 idle = 0;
+                if (end) continue;
             }
-            if (have && gs - gp < 2 && (!need_q || test(C::B_QFULL + n_q % C::QB, (n_q / C::QB) & 1)) &&
-                test(C::B_KFULL + gs % NS, (gs / NS) & 1) &&
-                // S buffer gs & 1: the P V that reads chunk gs - 2's weights there is done (the last one
-                // issued is that one or a later one)
-                (gs < 2 || test(C::B_PVDONE, (gp - 1) & 1))) {
+            if (have && (!need_q || test(C::B_QFULL + n_q % C::QB, (n_q / C::QB) & 1)) &&
+                test(C::B_KFULL + gs % NS, (gs / NS) & 1)) {
                 need_q = false;
-                const int st = gs % NS, qb = n_q % C::QB;
-                const volatile Chunk& ck = sm.chunk[gs % ND];
-                const bool last = (__shfl_sync(0xffffffffu, ck.flags, 0) & LAST) != 0;
-                const int steps = __shfl_sync(0xffffffffu, ck.steps, 0);
-                tc_fence_after();
-                const uint32_t qs = smem_u32(sQ) + qb * C::Q_BYTES, ks = smem_u32(sK) + st * C::K_BYTES;
-#pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk)  // 16 values of the head: 32 B of a 64-wide part
-                    mma_f16_ss_if(one && kk < n16, tm + (uint32_t)((gs & 1) * KC),
-                                  smem_desc_sw128(qs + (kk >> 2) * QT * 128) + (uint64_t)(2 * (kk & 3)),
-                                  smem_desc_sw128(ks + (kk >> 2) * KC * 128) + (uint64_t)(2 * (kk & 3)), s_desc, kk != 0);
-                if (one) {
-                    mma_commit(bar(C::B_SFULL + (gs & 1)));
-                    mma_commit(bar(C::B_KFREE + st));
-                    if (last) mma_commit(bar(C::B_QFREE + qb));
-                }
-                if (gs & 1) steps_of[1] = steps;
-                else steps_of[0] = steps;
-                firsts = (firsts & ~(1u << (gs & 3))) | (uint32_t)first << (gs & 3);
-                first = false;
-                ++gs;
-                if (last) {
-                    have = false;
-                    ++n_q;
-                }
+                issue_s();
                 idle = 0;
+                continue;
             }
             if (gp < gs && test(C::B_PFULL + (gp & 1), (gp >> 1) & 1) && test(C::B_VFULL + gp % NS, (gp / NS) & 1)) {
-                const int st = gp % NS, steps = gp & 1 ? steps_of[1] : steps_of[0];
-                tc_fence_after();
-                const uint64_t vd = v_desc(smem_u32(sV) + st * C::K_BYTES, KC * 128);
-                const bool over = firsts >> (gp & 3) & 1u;
-#pragma unroll
-                for (int j = 0; j < KC / 16; ++j)  // 16 keys: 2048 B of V, 8 columns of P
-                    mma_f16_ts_if(one && j < steps, tm + C::O_COL, tm + (uint32_t)((gp & 1) * KC + 8 * j),
-                                  vd + (uint64_t)(128 * j), o_desc, !(over && j == 0));
-                if (one) {
-                    mma_commit(bar(C::B_PVDONE));
-                    mma_commit(bar(C::B_VFREE + st));
-                }
-                ++gp;
+                issue_pv();
+                if (!(ok = wait_warp(C::B_PVDONE + ((gp - 1) & 1), ((gp - 1) >> 1) & 1))) break;
                 idle = 0;
+                continue;
             }
-            if (end && gp == gs) break;
             if (idle == 0) t0 = (uint32_t)clock();
-            if ((idle & 255) == 255) {  // bounded, as every wait
-                if (__any_sync(0xffffffffu, wait_over(abort, a.err, t0, C::B_DRAIN))) break;
-            }
+            if ((idle & 255) == 255)  // bounded, as every wait
+                ok = !__any_sync(0xffffffffu, wait_over(abort, a.err, t0, C::B_DRAIN));
         }
         if (one) mma_commit(bar(C::B_DRAIN));  // every MMA issued has finished before TMEM is freed
         mbar_wait(bar(C::B_DRAIN), 0, nullptr, nullptr, 0);
@@ -652,9 +673,8 @@ __global__ void __launch_bounds__(NTHR, 2)
         bool ok = true;
         // V rows past the sequence's end hold other rows of the buffer: cleared
         auto clear_v = [&](int k0, int m) {
-            if (k0 + KC <= m) return true;
             const int st = g % NS;
-            if (!wait_warp(C::B_VFULL + st, (g / NS) & 1)) return false;
+            if (!wait_at(C::B_VFULL + st, (g / NS) & 1)) return false;
             if (row < KC && k0 + row >= m) {
 #pragma unroll
                 for (int x = 0; x < HD / 64; ++x)
@@ -688,16 +708,11 @@ __global__ void __launch_bounds__(NTHR, 2)
             if (!__any_sync(0xffffffffu, live)) {
                 // none of the warp's rows is one: it keeps to the barriers and its share of V
                 for (bool last = empty; !last; ++g) {
-                    const int ds = g % ND;
-                    if (!(ok = wait_warp(C::B_CHUNK + ds, (g / ND) & 1) &&
-                               wait_warp(C::B_SFULL + (g & 1), (g >> 1) & 1)))
-                        break;
-                    const int k0 = sm.chunk[ds].k0;
-                    last = (sm.chunk[ds].flags & LAST) != 0;
-                    if (!(ok = clear_v(k0, s.m))) break;
+                    if (!(ok = wait_warp(C::B_SFULL + (g & 1), (g >> 1) & 1))) break;
+                    const Chunk ck = sm.now[g & 1];
+                    last = (ck.flags & LAST) != 0;
+                    if ((ck.flags & TAIL) && !(ok = clear_v(ck.k0, s.m))) break;
                     __syncwarp();
-                    // (as the others: a phase of P V is waited for before the next may complete)
-                    if (g > 0 && !(ok = wait_warp(C::B_PVDONE, (g - 1) & 1))) break;
                     if (lane == 0) mbar_arrive(bar(C::B_PFULL + (g & 1)));
                     __syncwarp();
                 }
@@ -709,18 +724,18 @@ __global__ void __launch_bounds__(NTHR, 2)
             }
             float m_run = -INFINITY, l_run = 0.0f;  // the maximum in use (log2 units) and the sum
             for (bool first = true; !empty; first = false) {
-                const int ds = g % ND;
-                if (!(ok = wait_warp(C::B_CHUNK + ds, (g / ND) & 1) &&
-                           wait_warp(C::B_SFULL + (g & 1), (g >> 1) & 1)))
-                    break;
+                // (a wait that failed shows at the chunk's end: what is computed then goes nowhere)
+                ok = wait_at(C::B_SFULL + (g & 1), (g >> 1) & 1);
                 tc_fence_after();
-                const Chunk ck = sm.chunk[ds];
-                const int k0 = ck.k0, flags = ck.flags;
+                const Chunk& ck = sm.now[g & 1];
+                const int flags = ck.flags;
                 const uint32_t s_t = row_t + (uint32_t)((g & 1) * KC);
-                if (!(ok = clear_v(k0, s.m))) break;
                 Words seen;
-                if (flags & MASKED) seen = seen_chunk<KC>(a, s, place, k0, doc, flags & DOCS ? sm.docs[ds] : nullptr);
-                const int d0 = k0 - place;
+                if (flags & MASKED) {
+                    if (flags & TAIL) ok &= clear_v(ck.k0, s.m);
+                    seen = seen_chunk<KC>(a, s, place, ck.k0, doc, flags & DOCS ? sm.docs[ck.docs] : nullptr);
+                }
+                const int d0 = KIND == PLAIN ? 0 : ck.k0 - place;
                 if constexpr (KIND == ANY) prepare_scores<KC>(a, s_t, d0, scale2, slope2, table);
                 uint32_t v[KC];
                 auto load = [&] {
@@ -781,31 +796,28 @@ __global__ void __launch_bounds__(NTHR, 2)
                     f2_unpack(f2_add(sum[0], sum[1]), s0, s1);
                     l_run = l_run * alpha + (s0 + s1);
                 }
-                if (g > 0) {
-                    // P V of chunk g - 1 has added to O (waited for in every chunk: no phase is left out)
-                    if (!(ok = wait_warp(C::B_PVDONE, (g - 1) & 1))) break;
+                if (raise && !first) {  // O, once P V of chunk g - 1 has added to it
+                    ok &= wait_at(C::B_PVDONE + ((g - 1) & 1), ((g - 1) >> 1) & 1);
                     tc_fence_after();
-                    if (raise && !first) {
 #pragma unroll 1
-                        for (int o0 = 0; o0 < HD; o0 += 32) {
-                            uint32_t ov[32];
-                            tmem_ld32(row_t + C::O_COL + (uint32_t)o0, ov);
-                            tmem_ld_wait();
+                    for (int o0 = 0; o0 < HD; o0 += 32) {
+                        uint32_t ov[32];
+                        tmem_ld32(row_t + C::O_COL + (uint32_t)o0, ov);
+                        tmem_ld_wait();
 #pragma unroll
-                            for (int t = 0; t < 32; ++t) ov[t] = __float_as_uint(__uint_as_float(ov[t]) * alpha);
-                            tmem_st32(row_t + C::O_COL + (uint32_t)o0, ov);
-                        }
+                        for (int t = 0; t < 32; ++t) ov[t] = __float_as_uint(__uint_as_float(ov[t]) * alpha);
+                        tmem_st32(row_t + C::O_COL + (uint32_t)o0, ov);
                     }
                 }
                 tmem_st_wait();
                 tc_fence_before();
-                __syncwarp();
+                if (!(ok = __all_sync(0xffffffffu, ok) != 0)) break;
                 if (lane == 0) mbar_arrive(bar(C::B_PFULL + (g & 1)));
                 ++g;
                 if (flags & LAST) break;
             }
             // the item's last P V has finished: O / sum
-            ok = ok && (empty || wait_warp(C::B_PVDONE, (g - 1) & 1));
+            ok = ok && (empty || wait_warp(C::B_PVDONE + ((g - 1) & 1), ((g - 1) >> 1) & 1));
             if (!ok) break;
             tc_fence_after();
             if constexpr (SPLIT) {

@@ -15,6 +15,12 @@ def unit(dtype):
     return torch.finfo(dtype).eps / 2
 
 
+def rounding(dtype, x):
+    """How far rounding to `dtype` may move x: half a step.  A step is eps of the value down to the
+    type's least normal number 2^e and stays eps 2^e below it (fp16: 2^-24, so half is 2^-25)."""
+    return unit(dtype) * x.abs().clamp(min=torch.finfo(dtype).smallest_normal)
+
+
 # ------------------------------------------------------------------ attention
 def attention(q, k, v, lens_q, lens_k, scale, softcap=0.0, window=(-1, -1), prefix=None, doc_q=None, doc_k=None,
               slopes=None, rel_bias=None):
@@ -22,7 +28,7 @@ def attention(q, k, v, lens_q, lens_k, scale, softcap=0.0, window=(-1, -1), pref
 
     The bound: the output's rounding, the weights' rounding (each weight times |v|), and the
     scores' error d, which moves every weight by a factor of at most e^(2d)."""
-    u = unit(q.dtype)
+    dtype, u = q.dtype, unit(q.dtype)
     q, k, v = (x.detach().cpu().to(F64) for x in (q, k, v))
     host = [None if x is None else x.detach().cpu() for x in (prefix, doc_q, doc_k, slopes, rel_bias)]
     prefix, doc_q, doc_k, slopes, rel_bias = host
@@ -75,7 +81,7 @@ def attention(q, k, v, lens_q, lens_k, scale, softcap=0.0, window=(-1, -1), pref
             d = near.amax(-1, keepdim=True) if m else torch.zeros(n, 1, dtype=F64)
             tiny = 2.0 ** -24 * (vs.abs().amax() if m else 0.0)  # weights below the type's least step
             out[at_q : at_q + n, h] = o
-            tol[at_q : at_q + n, h] = u * o.abs() + (u + torch.expm1(2 * d) + 2.0 ** -20) * size * (1 + u) + tiny
+            tol[at_q : at_q + n, h] = rounding(dtype, o) + (u + torch.expm1(2 * d) + 2.0 ** -20) * size * (1 + u) + tiny
         at_q, at_k = at_q + n, at_k + m
     return out, tol
 
@@ -108,7 +114,7 @@ def frequencies(rot, theta=10000.0, scaling="none", factor=1.0, context=0, beta_
 def rope(x, positions, rot, interleaved, freq, stretch):
     """(out, bound): sin and cos of a 64-bit angle reduced to fp32 (off by 2^-22), three fp32
     operations on each value, the output's rounding."""
-    u = unit(x.dtype)
+    dtype = x.dtype
     x = x.detach().cpu().to(F64)
     ang = positions.cpu().to(F64)[:, None] * freq
     c, s = (torch.cos(ang) * stretch)[:, None], (torch.sin(ang) * stretch)[:, None]
@@ -118,7 +124,7 @@ def rope(x, positions, rot, interleaved, freq, stretch):
     out[..., a] = x[..., a] * c - x[..., b] * s
     out[..., b] = x[..., a] * s + x[..., b] * c
     size[..., a] = size[..., b] = (x[..., a].abs() + x[..., b].abs()) * stretch
-    return out, u * out.abs() + 2.0 ** -20 * size
+    return out, rounding(dtype, out) + 2.0 ** -20 * size
 
 
 # ------------------------------------------------------------------ the linear layer
@@ -147,4 +153,4 @@ def linear(x, w, bias, act, residual, out_dtype, weights_rounded):
     if residual is not None:
         r = residual.cpu().to(F64)
         y, tol = y + r, tol + 2.0 ** -23 * (r.abs() + y.abs())
-    return y, tol + unit(out_dtype) * (y.abs() + tol)
+    return y, tol + rounding(out_dtype, y.abs() + tol)

@@ -15,6 +15,11 @@ pytestmark = pytest.mark.gpu
 BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
 
 
+@pytest.fixture(autouse=True)
+def _seed():
+    torch.manual_seed(6)
+
+
 def _cu(lens, dev):
     return torch.tensor([0] + list(np.cumsum(lens)), dtype=torch.int32, device=dev)
 
