@@ -198,12 +198,19 @@ def _vector(t, dtype, n: int, what: str):
         raise CrispEmbedError(f"{what}: {n} contiguous values of {dtype} expected")
 
 
-def _call_on(torch, dev: int, stream, call):
-    """call(stream pointer) with device `dev` current, on its current stream unless one is given."""
+def _raw_stream(torch, dev: int) -> int:
+    """The current stream of device `dev` as a pointer (the quick form where torch has it)."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(dev) if raw is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
+def _call_on(torch, dev: int, stream, fn, *args) -> int:
+    """fn(*args, stream pointer) with device `dev` current, on its current stream unless one is given."""
+    st = _raw_stream(torch, dev) if stream is None else int(stream)
     if torch.cuda.current_device() == dev:
-        return call(torch.cuda.current_stream(dev).cuda_stream if stream is None else int(stream))
+        return fn(*args, st)
     with torch.cuda.device(dev):
-        return call(torch.cuda.current_stream(dev).cuda_stream if stream is None else int(stream))
+        return fn(*args, st)
 
 
 class CrispEmbed:
@@ -495,16 +502,16 @@ class Linear:
         dev = _same_device("fused", x, (bias, residual, out))
         _vector(bias, torch.float32, n, "fused: bias")
         if out is None:
-            out = torch.empty((m, n), dtype=out_dtype or torch.float16, device=x.device)
+            out = x.new_empty((m, n), dtype=out_dtype or torch.float16)
         elif out_dtype is not None and out.dtype != out_dtype:
             raise CrispEmbedError("fused: out is not of out_dtype")
         for t in (out,) if residual is None else (out, residual):
             if t.dtype not in types or t.shape != (m, n) or t.stride(1) != 1:
                 raise CrispEmbedError(f"fused: residual and out must be [{m}, {n}] in fp32, fp16 or bf16 with contiguous rows")
         res = (None, 0, 0) if residual is None else (residual.data_ptr(), types[residual.dtype], residual.stride(0))
-        rc = _call_on(torch, dev, stream, lambda st: lib.ceb_linear_fused(
-            self._h, x.data_ptr(), x.stride(0), m, None if bias is None else bias.data_ptr(), ACTIVATIONS[act], *res,
-            types[out.dtype], out.data_ptr(), out.stride(0), st))
+        rc = _call_on(torch, dev, stream, lib.ceb_linear_fused, self._h, x.data_ptr(), x.stride(0), m,
+                      None if bias is None else bias.data_ptr(), ACTIVATIONS[act], *res, types[out.dtype],
+                      out.data_ptr(), out.stride(0))
         if rc:
             _check(rc, "ceb_linear_fused")
         return out
@@ -609,7 +616,7 @@ def attention_masked(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, max_
     if max_k is None:
         max_k = int((cu_k[1:] - cu_k[:-1]).max().item()) if n else 0
     if out is None:
-        out = torch.empty((rows, n_head, hd), dtype=dtype, device=q.device)
+        out = q.new_empty((rows, n_head, hd))
     elif out.shape != q.shape or out.dtype != dtype:
         raise CrispEmbedError("attention_masked: out must have q's shape and type")
     rr, rh, r1 = out.stride()
@@ -620,8 +627,8 @@ def attention_masked(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, max_
                           window[1], 0 if prefix is None else prefix.data_ptr(), 0 if doc_q is None else doc_q.data_ptr(),
                           0 if doc_k is None else doc_k.data_ptr(), 0 if slopes is None else slopes.data_ptr(),
                           0 if rel_bias is None else rel_bias.data_ptr(), radius)
-    rc = _call_on(torch, dev, stream, lambda st: lib.ceb_attention_masked(p, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                                                          out.data_ptr(), st))
+    rc = _call_on(torch, dev, stream, lib.ceb_attention_masked, p, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  out.data_ptr())
     if rc:
         _check(rc, "ceb_attention_masked")
     return out
@@ -665,16 +672,15 @@ class Rope:
             n = cu_seqlens.numel() - 1
             _vector(cu_seqlens, torch.int32, n + 1, "Rope: cu_seqlens")
         if out is None:
-            out = torch.empty((rows, heads, hd), dtype=dtype, device=x.device)
+            out = x.new_empty((rows, heads, hd))
         elif out.shape != x.shape or out.dtype != dtype:
             raise CrispEmbedError("Rope: out must have x's shape and type")
         (xr, xh, x1), (rr, rh, r1) = x.stride(), out.stride()
         if (x1 != 1 or r1 != 1) and hd > 1:
             raise CrispEmbedError("Rope: the values of a head must be contiguous")
-        rc = _call_on(torch, dev, stream, lambda st: lib.ceb_rope_forward(
-            self._h, x.data_ptr(), out.data_ptr(), types[dtype], rows, heads, hd, xr, xh, rr, rh, interleaved,
-            None if positions is None else positions.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(), n,
-            pos_offset, st))
+        rc = _call_on(torch, dev, stream, lib.ceb_rope_forward, self._h, x.data_ptr(), out.data_ptr(), types[dtype], rows,
+                      heads, hd, xr, xh, rr, rh, interleaved, None if positions is None else positions.data_ptr(),
+                      None if cu_seqlens is None else cu_seqlens.data_ptr(), n, pos_offset)
         if rc:
             _check(rc, "ceb_rope_forward")
         return out

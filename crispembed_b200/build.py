@@ -22,7 +22,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libcrispembed.so")
 
 SOURCES = ["gemm_tc.cu", "linear_few.cu", "attn_tc.cu", "attn_fa.cu", "moe.cu", "moe_static.cu", "ep.cu", "encoder_kernels.cu", "ref_arith.cu", "rope.cu", "attn_masked.cu", "attn_masked_f16.cu", "attn_masked_bf16.cu", "runtime.cpp", "gguf_quants.cpp", "gguf.cpp", "tokenizer.cpp", "model.cpp", "api.cpp"]
-HEADERS = ["common.cuh", "attn_tile.cuh", "epilogue.cuh", "attn_masked.h", "rowwise.cuh", "ceb_internal.h", "ceb_moe_internal.h", "ceb_ep_internal.h", "ceb_encoder_internal.h", "gguf.h", "tokenizer.h", "spm_norm_table.inc",
+HEADERS = ["common.cuh", "attn_tile.cuh", "attn_few.cuh", "epilogue.cuh", "attn_masked.h", "rowwise.cuh", "ceb_internal.h", "ceb_moe_internal.h", "ceb_ep_internal.h", "ceb_encoder_internal.h", "gguf.h", "tokenizer.h", "spm_norm_table.inc",
            "ceb_portable_math.h"]
 PUBLIC_HEADERS = [os.path.join(ROOT, "include", h) for h in ("crispembed.h", "ceb_ops.h")]
 

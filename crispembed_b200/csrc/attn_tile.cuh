@@ -334,6 +334,52 @@ __device__ __noinline__ void prepare_scores(const Args& a, uint32_t s_t, int d0,
     tmem_st_wait();
 }
 
+// Weights for joining partial softmaxes, a lane each (`on`; maximum in log2 units and sum): f, the
+// lane's factor, and for all lanes the joint maximum and sum.  Returns the lanes that have seen
+// a key (of the others the O may be anything).
+CEB_DEV unsigned join_weights(bool on, float2 ml, float& f, float& top, float& sum) {
+    const bool none = !on || (ml.y == 0.0f && ml.x == -INFINITY);
+    top = none ? -INFINITY : ml.x;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    f = none ? 0.0f : top == -INFINITY ? 1.0f : ex2f(ml.x - top);
+    sum = none ? 0.0f : f * ml.y;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return __ballot_sync(0xffffffffu, !none);
+}
+// One row of the blocks of a cluster, by a warp: ml and o (fp32, HD values) lie at these places
+// in every block.  A lane gets four values of the head, and the sum.
+template <int HD, bool CLUSTER>
+CEB_DEV void join_row(const float2* ml, const void* o, int parts, float (&acc)[4], float& sum) {
+    const int lane = threadIdx.x & 31;
+    auto at = [&](const void* p, int c) { return CLUSTER ? mapa_shared(smem_u32(p), c) : smem_u32(p); };
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                 : "=f"(v.x), "=f"(v.y)
+                 : "r"(at(ml, min(lane, parts - 1)))
+                 : "memory");
+    float f, top;
+    const unsigned used = join_weights(lane < parts, v, f, top, sum);
+    acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+    for (int c0 = 0; c0 < parts; c0 += 4) {
+        float4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (4 * lane < HD)
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(x[k].x), "=f"(x[k].y), "=f"(x[k].z), "=f"(x[k].w)
+                             : "r"(at(o, min(c0 + k, parts - 1)) + 16 * lane)
+                             : "memory");
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float fc = __shfl_sync(0xffffffffu, f, c0 + k);
+            if (4 * lane < HD && (used >> (c0 + k) & 1u))
+                acc[0] += fc * x[k].x, acc[1] += fc * x[k].y, acc[2] += fc * x[k].z, acc[3] += fc * x[k].w;
+        }
+    }
+}
+
 // SPLIT: the keys of an item are divided among the blocks of a cluster, which join their
 // sums through distributed shared memory; one item a block.
 // KIND: what stands between products and scores.  One of them is done in the registers that
@@ -964,35 +1010,9 @@ __global__ void __launch_bounds__(NTHR, 2)
             Seq s;
             if (load_seq(a, seq, false, s) && i0 < s.n) {
                 const int rows = min(tile_rows, s.n - i0) * a.group;
-                const uint32_t ml = smem_u32(sm.ml), o = smem_u32(sK);
                 for (int r = part + parts * (warp - 4); r < rows; r += parts * 4) {
-                    float top = -INFINITY;
-                    for (int c = 0; c < parts; ++c) {
-                        float m;
-                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(m) : "r"(mapa_shared(ml + 8 * r, c)) : "memory");
-                        top = fmaxf(top, m);
-                    }
-                    float sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    for (int c = 0; c < parts; ++c) {
-                        float m, l;
-                        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
-                                     : "=f"(m), "=f"(l)
-                                     : "r"(mapa_shared(ml + 8 * r, c))
-                                     : "memory");
-                        // a part without keys has no sums (its tiles hold anything)
-                        if (l == 0.0f && m == -INFINITY) continue;
-                        const float w = top == -INFINITY ? 1.0f : ex2f(m - top);
-                        sum += w * l;
-                        if (4 * lane < HD) {
-                            float x[4];
-                            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                         : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
-                                         : "r"(mapa_shared(o + (r * HD + 4 * lane) * 4, c))
-                                         : "memory");
-    #pragma unroll
-                            for (int k = 0; k < 4; ++k) acc[k] += w * x[k];
-                        }
-                    }
+                    float acc[4], sum;
+                    join_row<HD, true>(sm.ml + r, sK + r * HD * 4, parts, acc, sum);
                     const int i = i0 + r / a.group, head = kvh * a.group + r % a.group;
                     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
                     bool wrong = sum != sum || sum == INFINITY;
@@ -1066,9 +1086,7 @@ int launch_tiles(const Args& a, cudaStream_t st) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = parts > 1 ? 1 : 0;
-    // (split items, few rows each, are bound by their keys' bytes: two kinds will do)
-    auto kernel = parts > 1 ? attn_tile_kernel<T, HD, KC, KIND == PLAIN ? PLAIN : ANY, true>
-                           : attn_tile_kernel<T, HD, KC, KIND, false>;
+    auto kernel = parts > 1 ? attn_tile_kernel<T, HD, KC, KIND, true> : attn_tile_kernel<T, HD, KC, KIND, false>;
     if (int rc = ceb_func_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
     cudaError_t e = cudaSuccess;
     CEB_LAUNCH(CEB_PROF_ATTN, st, 0.0, 0.0,
