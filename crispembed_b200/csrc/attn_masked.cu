@@ -20,9 +20,10 @@ extern "C" int ceb_attention_masked(const ceb_attn_params* p, const void* d_q, c
         return ceb_set_error(2, "attention_masked: head_dim %d (a multiple of 8 up to 128)", p->head_dim);
     if (p->n_seqs < 0 || p->q_rows < 0 || p->k_rows < 0 || p->max_q < 0 || p->max_k < 0)
         return ceb_set_error(1, "attention_masked: negative count");
-    if (!std::isfinite(p->scale)) return ceb_set_error(1, "attention_masked: scale is not finite");
-    if (!(p->softcap >= 0.0f) || !std::isfinite(p->softcap))
-        return ceb_set_error(1, "attention_masked: softcap must be a finite number of at least 0");
+    // (what the kernels form of them, 2 scale log2(e) / softcap among it, stays finite)
+    if (!(std::fabs(p->scale) <= 1e15f)) return ceb_set_error(1, "attention_masked: scale beyond 1e15");
+    if (p->softcap != 0.0f && !(p->softcap >= 1e-15f && p->softcap <= 1e30f))
+        return ceb_set_error(1, "attention_masked: softcap must be 0 or 1e-15 to 1e30");
     if (p->window_left < -1 || p->window_right < -1)
         return ceb_set_error(1, "attention_masked: window sides are -1 (open) or a distance");
     if (!p->d_doc_q != !p->d_doc_k) return ceb_set_error(1, "attention_masked: documents of one side only");

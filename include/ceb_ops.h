@@ -293,7 +293,7 @@ CEB_API int ceb_attention_forward(const void* d_qkv, int n_rows, const int32_t* 
  * q [q_rows x n_head x head_dim], k and v [k_rows x n_head_kv x head_dim], out as q, all of
  * type dtype (CEB_ACT_F16 or CEB_ACT_BF16), 16-byte aligned, with strides in elements
  * that are multiples of 8 (values of a head are contiguous).  head_dim: a multiple of 8 up
- * to 128; n_head / n_head_kv <= 128.  max_q / max_k: at least the longest sequence of
+ * to 128; n_head / n_head_kv <= 128; |scale| up to 1e15, softcap 0 or 1e-15 to 1e30.  max_q / max_k: at least the longest sequence of
  * either side.  out may not overlap q, k or v; its rows that belong to no sequence stay as
  * they were.  Scores, softmax statistics and sums are fp32; the softmax weights meet V in
  * dtype.  No workspace, no state between calls: calls may overlap on any streams and may be

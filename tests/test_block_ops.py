@@ -43,6 +43,9 @@ def _attn(**kw):
     (dict(scale=float("inf")), 1),
     (dict(softcap=-1.0), 1),
     (dict(softcap=float("inf")), 1),
+    (dict(softcap=1e-16), 1),
+    (dict(softcap=2e30), 1),
+    (dict(scale=-2e15), 1),
     (dict(window_left=-2), 1),
     (dict(window_right=-2), 1),
     (dict(d_doc_q=P), 1),

@@ -254,6 +254,91 @@ def test_attention_long_single_token(cuda):
     _attend(q, k, v, [1] * 4, lens_k, window=(-1, 0), softcap=30.0)
 
 
+FEW = [dict(slopes=[0.1, 0.0, -0.02, 0.3]), dict(radius=40), dict(radius=700, softcap=3.0), dict(prefix=[7, 0, 64, 5]),
+       dict(docs=True), dict(softcap=2.0, scale=1.0), dict(scale=-0.2), dict(radius=9, low=True)]
+
+
+@pytest.mark.parametrize("kw", FEW)
+@pytest.mark.parametrize("hd", [40, 64, 128])
+@pytest.mark.parametrize("kv,most", [(4, 1), (1, 4), (2, 8)])
+def test_attention_few_rows(cuda, kw, hd, kv, most):
+    """Up to 16 rows a key head run on a kernel of their own: every mask and bias, keys that end inside
+    a step, sequences without rows or keys."""
+    lens_q, lens_k = [most, 1, 0, most], [333, 1, 64, 1030]
+    q, k, v = _qkv(cuda, BF if hd == 64 else HF, sum(lens_q), sum(lens_k), 4, kv, hd)
+    kw, n = dict(kw), sum(lens_k)
+    radius, docs, low = kw.pop("radius", None), kw.pop("docs", False), kw.pop("low", False)
+    if "slopes" in kw:
+        kw["slopes"] = torch.tensor(kw["slopes"], device=cuda)
+    if "prefix" in kw:
+        kw.update(prefix=torch.tensor(kw["prefix"], dtype=torch.int32, device=cuda), window=(30, 0))
+    if radius:
+        kw["rel_bias"] = torch.randn(4, 2 * radius + 1, device=cuda)
+        if low:
+            kw["rel_bias"][1] = -math.inf
+            kw["rel_bias"][2] = torch.finfo(FP).min
+    if docs:
+        kw["doc_k"] = torch.randint(-1, 3, (n,), device=cuda).int()
+        kw["doc_q"] = torch.randint(-1, 3, (sum(lens_q),), device=cuda).int()
+    _attend(q, k, v, lens_q, lens_k, **kw)
+
+
+@pytest.mark.parametrize("poison", [math.nan, math.inf])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_few_rows_hidden_keys(cuda, poison, hd):
+    lens_q, lens_k = [1, 3], [100, 4000]
+    q, k, v = _qkv(cuda, BF, 4, 4140, 4, 2, hd)
+    q2, k2, v2 = q.clone(), k.clone(), v.clone()
+    for t in (k2, v2):
+        t[100 + 3000:100 + 3100] = poison  # hidden by the window
+        t[4100:] = poison                  # behind the last sequence
+    cu = _cu(lens_q, cuda), _cu(lens_k, cuda)
+    kw = dict(window=(500, 0))
+    out = binding.attention_masked(q2, k2, v2, *cu, 3, 4000, **kw)
+    binding.sync_check()
+    ref, tol = R.attention(q, k[:4100], v[:4100], lens_q, lens_k, hd ** -0.5, **kw)
+    R.check(out, ref, tol)
+    v2[100 + 3990] = poison                # seen by the second text's rows
+    out = binding.attention_masked(q2, k2, v2, *cu, 3, 4000, **kw)
+    R.check(out[:1], ref[:1], tol[:1])
+    assert not torch.isfinite(out[1:]).any()
+
+
+def test_attention_few_rows_bad_offsets(cuda):
+    q, k, v = _qkv(cuda, HF, 2, 64, 2, 2, 64)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    for cu_k in ([0, 70, 64], [0, 30, 80], [-1, 30, 64]):
+        binding.attention_masked(q, k, v, t([0, 1, 2]), t(cu_k), 1, 64)
+        with pytest.raises(binding.CrispEmbedError, match=r"\(5\).*0x106"):
+            binding.sync_check()
+
+
+def test_first_call_of_a_process_is_captured(cuda):
+    """The library's device words may be made while the caller's stream is being captured."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from crispembed_b200 import binding
+q = torch.randn(70, 2, 64, device="cuda").half()
+cu = torch.tensor([0, 70], dtype=torch.int32, device="cuda")
+out = torch.zeros_like(q)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    binding.attention_masked(q, q, q, cu, cu, 70, 70, out=out)
+assert (out == 0).all()
+g.replay()
+ref = binding.attention_masked(q, q, q, cu, cu, 70, 70)
+binding.sync_check()
+assert torch.equal(out, ref) and (out != 0).any()
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_attention_repeats_overlaps_and_replays(cuda):
     """The same bits again; on two streams at once; captured by two graphs on one stream and
     replayed on two."""
