@@ -26,7 +26,9 @@ extern "C" int ceb_attention_masked(const ceb_attn_params* p, const void* d_q, c
         return ceb_set_error(1, "attention_masked: softcap must be 0 or 1e-15 to 1e30");
     if (p->window_left < -1 || p->window_right < -1)
         return ceb_set_error(1, "attention_masked: window sides are -1 (open) or a distance");
-    if (!p->d_doc_q != !p->d_doc_k) return ceb_set_error(1, "attention_masked: documents of one side only");
+    // (an empty side has no numbers to give)
+    if (!p->d_doc_q != !p->d_doc_k && p->q_rows > 0 && p->k_rows > 0)
+        return ceb_set_error(1, "attention_masked: documents of one side only");
     if (p->d_slopes && p->d_rel_bias) return ceb_set_error(1, "attention_masked: slopes and a bias table");
     if (p->d_rel_bias && (p->rel_bias_radius < 0 || p->rel_bias_radius > (1 << 24)))
         return ceb_set_error(1, "attention_masked: bias radius %d", p->rel_bias_radius);
@@ -72,8 +74,8 @@ extern "C" int ceb_attention_masked(const ceb_attn_params* p, const void* d_q, c
     a.cu_q = p->d_cu_q;
     a.cu_k = p->d_cu_k;
     a.prefix = p->d_prefix;
-    a.doc_q = p->d_doc_q;
-    a.doc_k = p->d_doc_k;
+    a.doc_q = p->k_rows > 0 ? p->d_doc_q : nullptr;
+    a.doc_k = p->k_rows > 0 ? p->d_doc_k : nullptr;
     a.slopes = p->d_slopes;
     a.table = p->d_rel_bias;
     a.n_head = p->n_head;

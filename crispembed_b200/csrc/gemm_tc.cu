@@ -39,7 +39,6 @@
 // stage; quantized planes are dequantized in shared memory as here.
 #include <cstdio>
 #include <cstdlib>
-#include <type_traits>
 
 #include "../../include/ceb_ops.h"
 #include "ceb_internal.h"

@@ -212,9 +212,12 @@ def test_attention_rows_of_no_sequence(cuda):
 def test_attention_no_key_rows(cuda):
     q = torch.randn(5, 2, 64, device=cuda).half()
     k = torch.empty(0, 2, 64, device=cuda).half()
-    out = binding.attention_masked(q, k, k, _cu([5], cuda), _cu([0], cuda), 5, 0)
-    binding.sync_check()
-    assert (out == 0).all()
+    doc = torch.zeros(5, dtype=torch.int32, device=cuda)
+    for kw in ({}, dict(doc_q=doc, doc_k=doc[:0])):
+        for rows in (5, 1):
+            out = binding.attention_masked(q, k, k, _cu([rows], cuda), _cu([0], cuda), rows, 0, out=torch.ones_like(q), **kw)
+            binding.sync_check()
+            assert (out[:rows] == 0).all() and (out[rows:] == 1).all()
 
 
 @pytest.mark.parametrize("cu_q,cu_k,max_q,max_k", [
