@@ -223,9 +223,11 @@ __global__ void __launch_bounds__(32 * FW, 2)
                 const float nm = UP<T> - (m_run[h] == -INFINITY ? 0.0f : m_run[h]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[h][e] = ex2f(w[h][e] + nm);
-                l_run[h] += (w[h][0] + w[h][1]) + (w[h][2] + w[h][3]);
                 pa[h] = pack(w[h][0], w[h][1], T());
                 pa[2 + h] = pack(w[h][2], w[h][3], T());
+                float s0, s1;
+                f2_unpack(f2_add(unpack(pa[h], T()), unpack(pa[2 + h], T())), s0, s1);
+                l_run[h] += s0 + s1;
             }
 #pragma unroll
             for (int n = 0; n < HD / 16; ++n) {  // 16 head values: four 8x8 tiles (keys 0-7, 8-15) x two pieces
