@@ -554,9 +554,12 @@ __global__ void __launch_bounds__(NTHR, 2)
                 dq1 = __reduce_max_sync(0xffffffffu, dq1);
             }
             // The next of the positions from `at` on whose chunk holds a document of the tile.  Ranges of
-            // eight chunks are found at a time and kept for the sequence's other tiles and heads.
+            // eight chunks are found at a time and kept for the sequence's other tiles and heads.  A slot
+            // serves every 256th chunk and may change hands as the search goes on, so a lane takes its
+            // position's range into registers while the slot is known to hold it.
             unsigned hits = 0;  // those of positions from hits_at on
             int hits_at = -32;
+            int2 docs_of = make_int2(0, 0);  // of the chunk at position hits_at + lane
             auto seek = [&](int at) {
                 if (at < hits_at + 32) {
                     const unsigned ahead = hits >> (at - hits_at);
@@ -600,9 +603,9 @@ __global__ void __launch_bounds__(NTHR, 2)
                         if (lane == 0) sm.range_tag[b % (RANGES / 8)] = b;
                         __syncwarp();
                     }
-                    const int2 r = sm.range[c % RANGES];
+                    docs_of = sm.range[c % RANGES];
                     hits = __ballot_sync(
-                        0xffffffffu, p < t_end && r.x <= dq1 && (r.y < 0 ? -1 - r.y : r.y) >= dq0);
+                        0xffffffffu, p < t_end && docs_of.x <= dq1 && (docs_of.y < 0 ? -1 - docs_of.y : docs_of.y) >= dq0);
                     hits_at = at;
                     if (hits) return at + __ffs(hits) - 1;
                 }
@@ -610,9 +613,15 @@ __global__ void __launch_bounds__(NTHR, 2)
             };
             // positions t .. t_end - 1; a chunk is loaded once it is known whether another follows
             const int qb = n_q % C::QB;
-            int pend = -1;  // the chunk to load
+            int pend = -1;                   // the chunk to load
+            int2 pend_docs = docs_of;        // and its range of documents
             for (bool more = true; more; ++t) {
-                if (a.doc_k) t = seek(t);
+                int2 t_docs = docs_of;
+                if (a.doc_k) {
+                    t = seek(t);
+                    t_docs.x = __shfl_sync(0xffffffffu, docs_of.x, t - hits_at);  // (no chunk at t_end: not used)
+                    t_docs.y = __shfl_sync(0xffffffffu, docs_of.y, t - hits_at);
+                }
                 more = t < t_end;
                 const int k0 = more ? chunk_at(t) * KC : 0;
                 if (pend < 0) {  // the first chunk, or that there is none
@@ -636,9 +645,8 @@ __global__ void __launch_bounds__(NTHR, 2)
                     int flags = (more ? 0 : LAST) | (j0 + KC > s.m ? TAIL : 0), docs = 0;
                     if (j0 + KC > s.m || !(j0 + KC <= s.prefix || (j0 >= lo1 && j0 + KC <= hi0))) flags |= MASKED;
                     if (a.doc_k) {
-                        const int2 r = sm.range[j0 / KC % RANGES];
-                        if (r.x == r.y) {  // keys of one document
-                            docs = r.x;
+                        if (pend_docs.x == pend_docs.y) {  // keys of one document
+                            docs = pend_docs.x;
                             if (q_none || dq0 != dq1 || dq0 != docs) flags |= MASKED | ONE_DOC;
                         } else {
                             docs = ds;
@@ -672,6 +680,7 @@ __global__ void __launch_bounds__(NTHR, 2)
                     __syncwarp();
                 }
                 pend = k0;
+                pend_docs = t_docs;
             }
         }
         if (ok) {
