@@ -573,10 +573,19 @@ __global__ void __launch_bounds__(NTHR, 2)
                 }
                 for (; at < t_end; at += 32) {
                     const int p = at + lane, c = chunk_at(p < t_end ? p : at);  // this lane's chunk
-                    for (unsigned need;;) {  // blocks of eight that are not there yet
-                        const int tag = c >> 3, slot = tag % (RANGES / 8);
-                        need = __ballot_sync(0xffffffffu, p < t_end && sm.range_tag[slot] != tag);
+                    // A lane takes its range as soon as its slot holds it, then blocks of eight that are not
+                    // there are fetched: the first waiting lane's each time, so 32 at most.  (Where positions
+                    // jump from the prefix to the windows or wrap at the end, two lanes may want one slot for
+                    // blocks of their own; both there at once they never are.)
+                    bool want = p < t_end;
+                    for (const int tag = c >> 3;;) {
+                        if (want && sm.range_tag[tag % (RANGES / 8)] == tag) {
+                            docs_of = sm.range[c % RANGES];
+                            want = false;
+                        }
+                        const unsigned need = __ballot_sync(0xffffffffu, want);
                         if (!need) break;
+                        __syncwarp();  // the slots have been read
                         const int b = __shfl_sync(0xffffffffu, tag, __ffs(need) - 1);
                         int d[8][KC / 32];
 #pragma unroll
@@ -603,7 +612,6 @@ __global__ void __launch_bounds__(NTHR, 2)
                         if (lane == 0) sm.range_tag[b % (RANGES / 8)] = b;
                         __syncwarp();
                     }
-                    docs_of = sm.range[c % RANGES];
                     hits = __ballot_sync(
                         0xffffffffu, p < t_end && docs_of.x <= dq1 && (docs_of.y < 0 ? -1 - docs_of.y : docs_of.y) >= dq0);
                     hits_at = at;

@@ -23,7 +23,7 @@ class Warp:
         self.true = np.stack([least, np.where((keys < 0).any(1), -1 - most.clip(min=0), most)], 1)
         self.tag = np.full(RANGES // 8, -1)
         self.range = np.zeros((RANGES, 2), dtype=np.int64)
-        self.filled = 0  # most blocks of eight fetched for one step of 32
+        self.filled = 0  # most blocks of eight fetched for a step of 32 positions
 
     def span(self, place):
         """The window of the row at `place`."""
@@ -92,14 +92,19 @@ class Warp:
             pend, t = found, t + 1
 
     def step(self, c, on):
-        """The ranges of the lanes' chunks c (where `on`)."""
-        blocks = 0
-        while (need := on & (self.tag[(c >> 3) % (RANGES // 8)] != c >> 3)).any():
-            self.fetch(int((c >> 3)[need.argmax()]))
+        """The ranges of the lanes' chunks c (where `on`): a lane takes its own while its slot holds it."""
+        want, got, blocks = on.copy(), np.zeros((32, 2), dtype=np.int64), 0
+        while True:
+            there = want & (self.tag[(c >> 3) % (RANGES // 8)] == c >> 3)
+            got[there] = self.range[c % RANGES][there]
+            want &= ~there
+            if not want.any():
+                break
+            self.fetch(int((c >> 3)[want.argmax()]))
             blocks += 1
-            assert blocks <= 32, "two lanes need one slot"
+            assert blocks <= 32, "the search does not end"
         self.filled = max(self.filled, blocks)
-        return self.range[c % RANGES]
+        return got
 
     def seen(self, i0, visits):
         """What the tile's rows see, [rows, keys]: windows and prefix, and documents by the chunk's flags."""

@@ -36,3 +36,21 @@ def test_documents_of_few_rows(rows, keys, parts):
     doc = documents(keys, "runs")
     doc_q = doc[np.linspace(0, keys - 1, rows).astype(int)]
     _check(Warp(doc_q, doc, 64, 64), rows, 64, parts=parts)
+
+
+JUMPS = [  # (window, prefix, the nearest chunk first): positions that are not neighbouring chunks
+    ((-1, -1), 0, True), ((-1, 0), 0, True), ((1024, 0), 100, False), ((1024, 0), 1000, False), ((1024, 0), 1000, True),
+    ((300, 300), 9000, True), ((300, 5), 16380, False),
+]
+
+
+@pytest.mark.parametrize("keys", [500, 16385, 17000, 20000, 33500])
+@pytest.mark.parametrize("chunk", [64, 96])
+@pytest.mark.parametrize("window,prefix,near_first", JUMPS)
+@pytest.mark.parametrize("kind", ["runs", "shuffled"])
+def test_search_ends_where_positions_jump(keys, chunk, window, prefix, near_first, kind):
+    """Two of a step's 32 positions may want the same slot for chunks 256 apart."""
+    doc = documents(keys, kind)
+    warp = Warp(doc, doc, chunk, 128, window, prefix, near_first)
+    _check(warp, keys, 128)
+    assert warp.filled <= 7  # 32 positions in up to two runs, each of which may begin inside a block

@@ -42,6 +42,25 @@ def test_documents_of_long_rows(cuda, dtype, hd, heads, kv, keys, kw, kind):
     _attend(cuda, dtype, keys, keys, heads, kv, hd, kind, **kw)
 
 
+@pytest.mark.parametrize("dtype,hd,keys,bias,kw", [
+    (HF, 64, 17000, "slopes", {}),
+    (BF, 128, 18000, "table", {}),
+    (HF, 128, 33500, "slopes", dict(window=(-1, 0))),
+    (BF, 64, 20000, None, dict(window=(1024, 0), prefix=1000)),   # 96 keys a chunk: the positions jump
+    (HF, 96, 20000, None, dict(window=(1024, 0), prefix=100)),
+    (HF, 64, 20000, "table", dict(window=(300, 300), prefix=9000)),
+])
+def test_documents_where_positions_jump(cuda, dtype, hd, keys, bias, kw):
+    """The chunk near a row comes first where there is a bias, and windows lie behind a prefix."""
+    g = torch.Generator().manual_seed(keys)
+    if bias == "slopes":
+        kw = dict(kw, slopes=torch.tensor([0.01, 0.0002], device=cuda))
+    if bias == "table":
+        kw = dict(kw, rel_bias=torch.randn(2, 201, generator=g).to(cuda))
+    for kind in ("runs", "far"):
+        _attend(cuda, dtype, keys, keys, 2, 1, hd, kind, **kw)
+
+
 @pytest.mark.parametrize("kind", ["runs", "far"])
 def test_documents_of_few_rows_and_many_keys(cuda, kind):
     """The keys of a tile divided among a cluster's blocks, more than 256 chunks each."""
