@@ -171,10 +171,15 @@ __global__ void __launch_bounds__(32 * FW, 2)
                     continue;
                 }
                 if (a.cap > 0.0f) {
-                    const float in = 2.0f * LOG2E * a.scale / a.cap, up = a.cap * LOG2E;
+                    const float in = a.scale / a.cap;
+                    float top = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        w[h][e] = up * fmaf(-2.0f, rcpf(1.0f + ex2f(c[e >> 1][2 * h + (e & 1)] * in)), 1.0f);
+                    for (int e = 0; e < 4; ++e) {
+                        w[h][e] = c[e >> 1][2 * h + (e & 1)];
+                        top = fmaxf(top, fabsf(w[h][e] * in));
+                    }
+                    if (__all_sync(0xffffffffu, top <= 1.0f)) capped(w[h], in, scale2, a.cap * LOG2E, false);
+                    else capped(w[h], in, scale2, a.cap * LOG2E, true);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) w[h][e] = c[e >> 1][2 * h + (e & 1)] * scale2;

@@ -125,6 +125,39 @@ CEB_DEV float rcpf(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// c tanh(s / c) of the score s = x scale, y = s / c = x in.  Up to |y| = 1 it is s P(y^2), with P
+// fitted to tanh(y) / y on [0, 1] for least relative error (2e-7 in fp32): multiply-adds alone, and as
+// good at any cap.  Beyond, c (1 - 2 / (1 + e^2y)): two special-function results a score, right to
+// 2^-22 of c, which is too little for a score far below it (0.07 off at a cap of 10^6).  Scores and cap
+// may be in any units (scale2, cap2: log2).
+CEB_DEV f32x2 capped_near(f32x2 x, f32x2 in, f32x2 scale2) {
+    const f32x2 y = f2_mul(x, in), z = f2_mul(y, y);
+    f32x2 p = f2_splat(0.0010410225950181484f);
+    p = f2_fma(p, z, f2_splat(-0.0062033794820308685f));
+    p = f2_fma(p, z, f2_splat(0.020289981737732887f));
+    p = f2_fma(p, z, f2_splat(-0.05345702916383743f));
+    p = f2_fma(p, z, f2_splat(0.13325203955173492f));
+    p = f2_fma(p, z, f2_splat(-0.33332839608192444f));
+    p = f2_fma(p, z, f2_splat(0.9999999403953552f));
+    return f2_mul(f2_mul(x, scale2), p);
+}
+CEB_DEV float capped_far(float y, float cap2) { return cap2 * fmaf(-2.0f, rcpf(1.0f + ex2f(2.0f * LOG2E * y)), 1.0f); }
+// Products x, an even number, capped in place; `beyond`: some of them may be (the same bits if none is).
+template <int N>
+CEB_DEV void capped(float (&x)[N], float in, float scale2, float cap2, bool beyond) {
+#pragma unroll
+    for (int t = 0; t < N; t += 2) {
+        float a, b;
+        f2_unpack(capped_near(f2_pack(x[t], x[t + 1]), f2_splat(in), f2_splat(scale2)), a, b);
+        if (beyond) {
+            const float y0 = x[t] * in, y1 = x[t + 1] * in;
+            a = fabsf(y0) <= 1.0f ? a : capped_far(y0, cap2);
+            b = fabsf(y1) <= 1.0f ? b : capped_far(y1, cap2);
+        }
+        x[t] = a;
+        x[t + 1] = b;
+    }
+}
 CEB_DEV float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -179,12 +212,7 @@ CEB_DEV uint32_t span_bits(int lo, int hi, int at) {
 // Products of 16 keys, the first of them d0 behind the row's place, into scores in log2 units.
 CEB_DEV void score_piece(const Args& a, uint32_t (&v)[16], int d0, float scale2, float slope2, const float* table) {
     if (a.cap > 0.0f) {
-        const float in = 2.0f * scale2 / a.cap, up = a.cap * LOG2E;
-#pragma unroll
-        for (int t = 0; t < 16; ++t) {  // tanh y = 1 - 2 / (1 + e^2y)
-            const float e = ex2f(__uint_as_float(v[t]) * in);
-            v[t] = __float_as_uint(up * fmaf(-2.0f, rcpf(1.0f + e), 1.0f));
-        }
+        capped(reinterpret_cast<float(&)[16]>(v), a.scale / a.cap, scale2, a.cap * LOG2E, true);
     } else {
 #pragma unroll
         for (int t = 0; t < 16; ++t) v[t] = __float_as_uint(__uint_as_float(v[t]) * scale2);
@@ -236,39 +264,15 @@ CEB_DEV void scores_slopes(uint32_t (&v)[N], int d0, int side, float scale2, flo
         }
     }
 }
-// c tanh(s / c).  With every |s| of the warp's rows up to c, y P(y^2) with P fitted to tanh(y) / y
-// on [0, 1] for least relative error (2e-7 in fp32): multiply-adds alone.  Beyond,
-// 1 - 2 / (1 + e^2y), two special-function results a score.
+// A row's scores capped.  With every |s| of the warp's rows up to the cap the multiply-adds alone are
+// run.
 template <int N>
-CEB_DEV void scores_capped(uint32_t (&v)[N], float scale2, float cap2) {
-    const float in = scale2 / cap2;
+CEB_DEV void scores_capped(uint32_t (&v)[N], float in, float scale2, float cap2) {
     float top = 0.0f;
 #pragma unroll
     for (int t = 0; t < N; t += 2) top = max3(top, fabsf(__uint_as_float(v[t])), fabsf(__uint_as_float(v[t + 1])));
-    if (__all_sync(0xffffffffu, top * in <= 1.0f)) {
-        const f32x2 in2 = f2_splat(in), up2 = f2_splat(cap2);
-#pragma unroll
-        for (int t = 0; t < N; t += 2) {
-            const f32x2 y = f2_mul(f2_pack(__uint_as_float(v[t]), __uint_as_float(v[t + 1])), in2), z = f2_mul(y, y);
-            f32x2 p = f2_splat(0.0010410225950181484f);
-            p = f2_fma(p, z, f2_splat(-0.0062033794820308685f));
-            p = f2_fma(p, z, f2_splat(0.020289981737732887f));
-            p = f2_fma(p, z, f2_splat(-0.05345702916383743f));
-            p = f2_fma(p, z, f2_splat(0.13325203955173492f));
-            p = f2_fma(p, z, f2_splat(-0.33332839608192444f));
-            p = f2_fma(p, z, f2_splat(0.9999999403953552f));
-            float a, b;
-            f2_unpack(f2_mul(f2_mul(y, up2), p), a, b);
-            v[t] = __float_as_uint(a);
-            v[t + 1] = __float_as_uint(b);
-        }
-    } else {
-#pragma unroll
-        for (int t = 0; t < N; ++t) {
-            const float e = ex2f(__uint_as_float(v[t]) * (2.0f * LOG2E * in));
-            v[t] = __float_as_uint(cap2 * fmaf(-2.0f, rcpf(1.0f + e), 1.0f));
-        }
-    }
+    if (__all_sync(0xffffffffu, top * in <= 1.0f)) capped(reinterpret_cast<float(&)[N]>(v), in, scale2, cap2, false);
+    else capped(reinterpret_cast<float(&)[N]>(v), in, scale2, cap2, true);
 }
 // Bias by distance from the head's table.  False (v then holds nothing) if an entry times log2 e
 // passes the lowest number.
@@ -899,7 +903,7 @@ __global__ void __launch_bounds__(NTHR, 2)
                     const int side = __all_sync(0xffffffffu, d0 >= 0) ? 1 : __all_sync(0xffffffffu, d0 + KC - 1 <= 0) ? -1 : 0;
                     scores_slopes(v, d0, side, scale2, slope2);
                 }
-                if constexpr (KIND == CAPPED) scores_capped(v, scale2, a.cap * LOG2E);
+                if constexpr (KIND == CAPPED) scores_capped(v, a.scale / a.cap, scale2, a.cap * LOG2E);
                 if constexpr (KIND == TABLE)
                     if (!scores_table(v, d0, a.radius, scale2, table)) {
                         prepare_scores<KC>(a, s_t, d0, scale2, slope2, table);
