@@ -920,12 +920,13 @@ __global__ void __launch_bounds__(NTHR, 2)
                     mx[(t >> 1) & 3] = max3(mx[(t >> 1) & 3], __uint_as_float(v[t]), __uint_as_float(v[t + 1]));
                 float cm = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
                 if (KIND == PLAIN) cm = cm == -INFINITY ? cm : cm * mul;  // (mul > 0)
-                const bool raise = __any_sync(0xffffffffu, cm > m_run + RAISE<T>) || first;
+                // A row raises its maximum for itself alone: other rows, be they of another sequence or none,
+                // and keys that only they see have no part in its bits.
+                const bool up = cm > m_run + RAISE<T>, raise = __any_sync(0xffffffffu, up && live);
                 float alpha = 1.0f;
-                if (raise) {
-                    const float m_new = fmaxf(m_run, cm);
-                    alpha = m_new == -INFINITY ? 1.0f : ex2f(m_run - m_new);
-                    m_run = m_new;
+                if (up) {
+                    alpha = ex2f(m_run - cm);
+                    m_run = cm;
                 }
                 const f32x2 nm2 = f2_splat(UP<T> - (m_run == -INFINITY ? 0.0f : m_run)), mul2 = f2_splat(mul);
                 f32x2 sum[2] = {f2_splat(0.0f), f2_splat(0.0f)};
