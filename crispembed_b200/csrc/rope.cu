@@ -276,7 +276,13 @@ extern "C" ceb_rope* ceb_rope_create(int rot_dim, double theta, int scaling, dou
     R->stretch = scaling == CEB_ROPE_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
     cudaError_t e = cudaGetDevice(&R->device);
     if (e == cudaSuccess) e = cudaMalloc(&R->turns, n * sizeof(double));
-    if (e == cudaSuccess) e = cudaMemcpy(R->turns, turns, n * sizeof(double), cudaMemcpyHostToDevice);
+    // On a stream of its own that is waited for: a copy on the legacy stream may return before it has
+    // landed, and streams that do not wait for that one could read the plan too early.
+    cudaStream_t own = nullptr;
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(R->turns, turns, n * sizeof(double), cudaMemcpyHostToDevice, own);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+    if (own) cudaStreamDestroy(own);
     if (e != cudaSuccess) {
         cudaGetLastError();
         ceb_set_cuda_error(e, "rope_create", __FILE__, __LINE__);
