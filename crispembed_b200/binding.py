@@ -198,6 +198,13 @@ def _vector(t, dtype, n: int, what: str):
         raise CrispEmbedError(f"{what}: {n} contiguous values of {dtype} expected")
 
 
+def _c_int(what: str, value: int) -> int:
+    """`value`, which a C int must hold: ctypes passes the lower 32 bits of any number."""
+    if not -(1 << 31) <= value < 1 << 31:
+        raise CrispEmbedError(f"{what}: {value} is not a 32-bit number")
+    return value
+
+
 def _raw_stream(torch, dev: int) -> int:
     """The current stream of device `dev` as a pointer (the quick form where torch has it)."""
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -622,11 +629,14 @@ def attention_masked(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, max_
     rr, rh, r1 = out.stride()
     if r1 != 1:
         raise CrispEmbedError("attention_masked: the values of a head must be contiguous")
-    p = _ATTN_PARAMS.pack(types[dtype], n_head, k.shape[1], hd, n, rows, keys, max_q, max_k, qr, qh, kr, kh, vr, vh, rr, rh,
-                          cu_q.data_ptr(), cu_k.data_ptr(), hd ** -0.5 if scale is None else scale, softcap, window[0],
-                          window[1], 0 if prefix is None else prefix.data_ptr(), 0 if doc_q is None else doc_q.data_ptr(),
-                          0 if doc_k is None else doc_k.data_ptr(), 0 if slopes is None else slopes.data_ptr(),
-                          0 if rel_bias is None else rel_bias.data_ptr(), radius)
+    try:
+        p = _ATTN_PARAMS.pack(types[dtype], n_head, k.shape[1], hd, n, rows, keys, max_q, max_k, qr, qh, kr, kh, vr, vh, rr, rh,
+                              cu_q.data_ptr(), cu_k.data_ptr(), hd ** -0.5 if scale is None else scale, softcap, window[0],
+                              window[1], 0 if prefix is None else prefix.data_ptr(), 0 if doc_q is None else doc_q.data_ptr(),
+                              0 if doc_k is None else doc_k.data_ptr(), 0 if slopes is None else slopes.data_ptr(),
+                              0 if rel_bias is None else rel_bias.data_ptr(), radius)
+    except (struct.error, OverflowError) as e:
+        raise CrispEmbedError(f"attention_masked: an argument does not fit its 32 bits ({e})") from None
     rc = _call_on(torch, dev, stream, lib.ceb_attention_masked, p, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   out.data_ptr())
     if rc:
@@ -648,8 +658,8 @@ class Rope:
         self._h = None
         self._lib = load_library()
         self.rot_dim = rot_dim
-        self._h = self._lib.ceb_rope_create(rot_dim, theta, ROPE_SCALINGS[scaling], factor, context, beta_fast,
-                                            beta_slow)
+        self._h = self._lib.ceb_rope_create(_c_int("Rope: rot_dim", rot_dim), theta, ROPE_SCALINGS[scaling], factor,
+                                            _c_int("Rope: context", context), beta_fast, beta_slow)
         if not self._h:
             raise CrispEmbedError(f"ceb_rope_create failed: {last_error()}")
 
@@ -662,8 +672,10 @@ class Rope:
         dtype = x.dtype
         if x.dim() != 3 or dtype not in types:
             raise CrispEmbedError("Rope: x must be [rows, heads, head_dim] in fp32, fp16 or bf16")
-        dev = _same_device("Rope", x, (out, positions, cu_seqlens))
+        _c_int("Rope: pos_offset", pos_offset)
         rows, heads, hd = x.shape
+        _c_int("Rope: rows", rows)
+        dev = _same_device("Rope", x, (out, positions, cu_seqlens))
         if positions is None and cu_seqlens is None:
             raise CrispEmbedError("Rope: positions or cu_seqlens must be given")
         n = 0
