@@ -64,9 +64,10 @@ CEB_DEV void store_f(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 // Row i of sequence s for one head, by one warp: a lane scores one key of 32, then every
 // lane carries the head's values lane, lane + 32, ...  Only keys that the row sees are read
 // into the sums, so what hidden keys hold cannot reach the result; one pass, with the
-// running maximum and sum of the softmax.
+// running maximum and sum of the softmax.  It takes its time (0.2 to 0.4 us a key): `beat`, if given, is
+// set to the clock all along, for waits that others bound.
 template <typename T>
-__device__ __noinline__ void warp_row(const Args& a, const Seq& s, int i, int head) {
+__device__ __noinline__ void warp_row(const Args& a, const Seq& s, int i, int head, volatile int* beat = nullptr) {
     const int lane = threadIdx.x & 31, hd = a.head_dim, kvh = head / a.group;
     const int p = i + s.m - s.n;
     int lo, hi;
@@ -81,6 +82,7 @@ __device__ __noinline__ void warp_row(const Args& a, const Seq& s, int i, int he
     // the keys of the prefix, then those of the window behind it
     int j0 = s.prefix > 0 ? 0 : lo / 32 * 32;
     while (j0 < max(hi, s.prefix)) {
+        if (beat && lane == 0) *beat = (int)clock();
         const int j = j0 + lane;
         bool seen = j < s.m && (j < s.prefix || (j >= lo && j < hi));
         if (seen && a.doc_k) seen = doc >= 0 && a.doc_k[s.k0 + j] == doc;

@@ -78,7 +78,7 @@ struct Small {  // shared memory behind the tiles
     uint64_t bars[MAX_BARS];
     alignas(16) uint32_t answer[4];
     uint32_t tmem;
-    int abort;
+    int abort[2];  // a role gave up; the clock when a row was last seen being computed again
     Item ring[NRING];
     Chunk chunk[MAX_ND];  // from the loading warp to the MMA warp
     Chunk now[2];         // of the S buffers, from there to the softmax
@@ -169,10 +169,12 @@ CEB_DEV uint32_t pack(float a, float b, __nv_bfloat16) {
     return *reinterpret_cast<uint32_t*>(&r);
 }
 // Whether a wait that began at clock t0 is over without its barrier: another role gave up, or
-// the time is up (about a second), which is recorded with the barrier's number.
+// the time is up (about a second, with no row computed again meanwhile), which is recorded with the
+// barrier's number.
 __device__ __noinline__ bool wait_over(volatile int* abort, int* err, uint32_t t0, int barrier) {
     if (*abort) return true;
-    if ((uint32_t)clock() - t0 < (uint32_t)CEB_WAIT_LIMIT_CYCLES) return false;
+    const uint32_t now = (uint32_t)clock(), limit = (uint32_t)CEB_WAIT_LIMIT_CYCLES;
+    if (now - t0 < limit || now - (uint32_t)abort[1] < limit) return false;
     *abort = 1;
     if (err) atomicCAS(err, 0, (int)CEB_DEVERR_TIMEOUT_MMA | ((barrier + 1) << 16));
     return true;
@@ -423,7 +425,8 @@ __global__ void __launch_bounds__(NTHR, 2)
         for (int i = 0; i < C::NBAR; ++i)
             mbar_init(smem_u32(&sm.bars[i]), (i == C::B_PFULL || i == C::B_PFULL + 1) ? 4 : (i == C::B_SFULL || i == C::B_SFULL + 1) ? 2 : (i >= C::B_IFREE ? 5 : 1));
         fence_mbar_init();
-        sm.abort = 0;
+        sm.abort[0] = 0;
+        sm.abort[1] = (int)clock();
         sm.now[0] = sm.now[1] = Chunk{0, 0, 0, 0};
     }
     if (warp == 0 && lane == 0) {
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(NTHR, 2)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
-    volatile int* abort = &sm.abort;
+    volatile int* abort = sm.abort;
     auto bar = [&](int i) { return smem_u32(&sm.bars[i]); };
     // Bounded waits; the error word names the barrier.  Most barriers are through when they are asked.
     auto wait_at = [&](int i, uint32_t par) {
@@ -1028,7 +1031,7 @@ __global__ void __launch_bounds__(NTHR, 2)
                 for (unsigned b = __ballot_sync(0xffffffffu, live && wrong); b; b &= b - 1) {
                     const int l = __ffs(b) - 1;
                     __syncwarp();
-                    warp_row<T>(a, s, __shfl_sync(0xffffffffu, i, l), __shfl_sync(0xffffffffu, head, l));
+                    warp_row<T>(a, s, __shfl_sync(0xffffffffu, i, l), __shfl_sync(0xffffffffu, head, l), abort + 1);
                 }
             }
             __syncwarp();

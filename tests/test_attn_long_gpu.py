@@ -65,3 +65,28 @@ def test_documents_where_positions_jump(cuda, dtype, hd, keys, bias, kw):
 def test_documents_of_few_rows_and_many_keys(cuda, kind):
     """The keys of a tile divided among a cluster's blocks, more than 256 chunks each."""
     _attend(cuda, HF, 200, 140000, 1, 1, 128, kind)
+
+
+def test_rows_of_a_long_text_computed_again(cuda):
+    """A hidden key that holds NaN: rows of 200,000 keys are computed again one by one, for longer than
+    the block's other warps wait for anything else, and the block has another text to do."""
+    n, keys, short = 600, 200000, 100
+    g = torch.Generator(device=cuda).manual_seed(2)
+    total = keys + (n - 1) * short
+    q = torch.randn(n, 32, 64, generator=g, device=cuda).half()
+    k, v = (torch.randn(total, 1, 64, generator=g, device=cuda).half() for _ in "kv")
+    doc_q = torch.zeros(n, dtype=torch.int32, device=cuda)
+    doc_k = torch.zeros(total, dtype=torch.int32, device=cuda)
+    doc_k[keys // 2] = -1
+    cu_q = torch.arange(n + 1, dtype=torch.int32, device=cuda)
+    cu_k = torch.cat([torch.zeros(1), keys + short * torch.arange(n)]).int().to(cuda)
+    ref = binding.attention_masked(q, k, v, cu_q, cu_k, 1, keys, doc_q=doc_q, doc_k=doc_k)
+    binding.sync_check()
+    v[keys // 2] = float("nan")
+    out = binding.attention_masked(q, k, v, cu_q, cu_k, 1, keys, doc_q=doc_q, doc_k=doc_k)
+    binding.sync_check()
+    assert torch.equal(out[1:], ref[1:])
+    v[keys // 2] = 0
+    want = attention_rows(q[:1], k[:keys], v[:keys], torch.arange(1), 0.125, doc_q=doc_q[:1], doc_k=doc_k[:keys])
+    R.check(ref[:1], *want)
+    R.check(out[:1], *want)
