@@ -171,15 +171,12 @@ __global__ void __launch_bounds__(32 * FW, 2)
                     continue;
                 }
                 if (a.cap > 0.0f) {
-                    const float in = a.scale / a.cap;
-                    float top = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        w[h][e] = c[e >> 1][2 * h + (e & 1)];
-                        top = fmaxf(top, fabsf(w[h][e] * in));
-                    }
-                    if (__all_sync(0xffffffffu, top <= 1.0f)) capped(w[h], in, scale2, a.cap * LOG2E, false);
-                    else capped(w[h], in, scale2, a.cap * LOG2E, true);
+                    for (int e = 0; e < 4; ++e) w[h][e] = c[e >> 1][2 * h + (e & 1)];
+                    const float in = a.scale / a.cap;
+                    const float top = fmaxf(max3(fabsf(w[h][0]), fabsf(w[h][1]), fabsf(w[h][2])), fabsf(w[h][3]));
+                    if (__all_sync(0xffffffffu, top * fabsf(in) <= 1.0f)) capped<NEAR, 4>(w[h], in, scale2, a.cap * LOG2E);
+                    else capped<EACH, 4>(w[h], in, scale2, a.cap * LOG2E);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) w[h][e] = c[e >> 1][2 * h + (e & 1)] * scale2;

@@ -125,37 +125,40 @@ CEB_DEV float rcpf(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// c tanh(s / c) of the score s = x scale, y = s / c = x in.  Up to |y| = 1 it is s P(y^2), with P
-// fitted to tanh(y) / y on [0, 1] for least relative error (2e-7 in fp32): multiply-adds alone, and as
-// good at any cap.  Beyond, c (1 - 2 / (1 + e^2y)): two special-function results a score, right to
-// 2^-22 of c, which is too little for a score far below it (0.07 off at a cap of 10^6).  Scores and cap
-// may be in any units (scale2, cap2: log2).
-CEB_DEV f32x2 capped_near(f32x2 x, f32x2 in, f32x2 scale2) {
-    const f32x2 y = f2_mul(x, in), z = f2_mul(y, y);
-    f32x2 p = f2_splat(0.0010410225950181484f);
-    p = f2_fma(p, z, f2_splat(-0.0062033794820308685f));
-    p = f2_fma(p, z, f2_splat(0.020289981737732887f));
-    p = f2_fma(p, z, f2_splat(-0.05345702916383743f));
-    p = f2_fma(p, z, f2_splat(0.13325203955173492f));
-    p = f2_fma(p, z, f2_splat(-0.33332839608192444f));
-    p = f2_fma(p, z, f2_splat(0.9999999403953552f));
-    return f2_mul(f2_mul(x, scale2), p);
-}
-CEB_DEV float capped_far(float y, float cap2) { return cap2 * fmaf(-2.0f, rcpf(1.0f + ex2f(2.0f * LOG2E * y)), 1.0f); }
-// Products x, an even number, capped in place; `beyond`: some of them may be (the same bits if none is).
-template <int N>
-CEB_DEV void capped(float (&x)[N], float in, float scale2, float cap2, bool beyond) {
+// c tanh(s / c) of the score s = x scale, y = s / c = x in.
+// NEAR, for |y| <= 1: s P(y^2), with P fitted to tanh(y) / y on [0, 1] for least relative error (2e-7 in
+//   fp32): multiply-adds alone, as good at any cap.
+// FAR: c (1 - 2 / (1 + e^2y)), two special-function results a score, right to 2^-22 of c.  Up to a cap
+//   of SMALL_CAP that is 2^-16 at most, a sixteenth of what rounding to fp16 does to a weight, and good
+//   for any score; at a cap of 10^6 a small score would be off by 0.07.
+// EACH: either one by the score's own y.
+// Scores and cap may be in any units (scale2, cap2: log2).
+enum { NEAR, FAR, EACH };
+constexpr float SMALL_CAP = 64.0f;
+template <int FORM, int N>
+CEB_DEV void capped(float* x, float in, float scale2, float cap2) {
 #pragma unroll
     for (int t = 0; t < N; t += 2) {
-        float a, b;
-        f2_unpack(capped_near(f2_pack(x[t], x[t + 1]), f2_splat(in), f2_splat(scale2)), a, b);
-        if (beyond) {
-            const float y0 = x[t] * in, y1 = x[t + 1] * in;
-            a = fabsf(y0) <= 1.0f ? a : capped_far(y0, cap2);
-            b = fabsf(y1) <= 1.0f ? b : capped_far(y1, cap2);
+        const f32x2 x2 = f2_pack(x[t], x[t + 1]), y = f2_mul(x2, f2_splat(in)), z = f2_mul(y, y);
+        if constexpr (FORM != FAR) {
+            f32x2 p = f2_splat(0.0010410225950181484f);
+            p = f2_fma(p, z, f2_splat(-0.0062033794820308685f));
+            p = f2_fma(p, z, f2_splat(0.020289981737732887f));
+            p = f2_fma(p, z, f2_splat(-0.05345702916383743f));
+            p = f2_fma(p, z, f2_splat(0.13325203955173492f));
+            p = f2_fma(p, z, f2_splat(-0.33332839608192444f));
+            p = f2_fma(p, z, f2_splat(0.9999999403953552f));
+            f2_unpack(f2_mul(f2_mul(x2, f2_splat(scale2)), p), x[t], x[t + 1]);
         }
-        x[t] = a;
-        x[t + 1] = b;
+        if constexpr (FORM != NEAR) {
+            float y0, y1, e0, e1;
+            f2_unpack(y, y0, y1);
+            f2_unpack(f2_mul(x2, f2_splat(2.0f * LOG2E * in)), e0, e1);
+            f2_unpack(f2_add(f2_pack(ex2f(e0), ex2f(e1)), f2_splat(1.0f)), e0, e1);
+            f2_unpack(f2_fma(f2_pack(rcpf(e0), rcpf(e1)), f2_splat(-2.0f * cap2), f2_splat(cap2)), e0, e1);
+            x[t] = FORM == EACH && fabsf(y0) <= 1.0f ? x[t] : e0;
+            x[t + 1] = FORM == EACH && fabsf(y1) <= 1.0f ? x[t + 1] : e1;
+        }
     }
 }
 CEB_DEV float max3(float a, float b, float c) {
@@ -214,7 +217,9 @@ CEB_DEV uint32_t span_bits(int lo, int hi, int at) {
 // Products of 16 keys, the first of them d0 behind the row's place, into scores in log2 units.
 CEB_DEV void score_piece(const Args& a, uint32_t (&v)[16], int d0, float scale2, float slope2, const float* table) {
     if (a.cap > 0.0f) {
-        capped(reinterpret_cast<float(&)[16]>(v), a.scale / a.cap, scale2, a.cap * LOG2E, true);
+        float* x = reinterpret_cast<float*>(v);
+        if (a.cap <= SMALL_CAP) capped<FAR, 16>(x, a.scale / a.cap, scale2, a.cap * LOG2E);
+        else capped<EACH, 16>(x, a.scale / a.cap, scale2, a.cap * LOG2E);
     } else {
 #pragma unroll
         for (int t = 0; t < 16; ++t) v[t] = __float_as_uint(__uint_as_float(v[t]) * scale2);
@@ -266,15 +271,19 @@ CEB_DEV void scores_slopes(uint32_t (&v)[N], int d0, int side, float scale2, flo
         }
     }
 }
-// A row's scores capped.  With every |s| of the warp's rows up to the cap the multiply-adds alone are
-// run.
+// A row's scores capped, where all of the warp's products are below the cap.  False (v as it was) if not:
+// prepare_capped then has the same bits for those that are.  4 x 4096 rows, 12 heads of 64: 623 us, where
+// scores pass the cap 896.  (FAR alone for these, by each row's own choice, would take 790, but its code
+// made the usual case 4 to 9 % slower.)
 template <int N>
-CEB_DEV void scores_capped(uint32_t (&v)[N], float in, float scale2, float cap2) {
+CEB_DEV bool scores_capped(uint32_t (&v)[N], float in, float scale2, float cap2) {
+    float* x = reinterpret_cast<float*>(v);
     float top = 0.0f;
 #pragma unroll
-    for (int t = 0; t < N; t += 2) top = max3(top, fabsf(__uint_as_float(v[t])), fabsf(__uint_as_float(v[t + 1])));
-    if (__all_sync(0xffffffffu, top * in <= 1.0f)) capped(reinterpret_cast<float(&)[N]>(v), in, scale2, cap2, false);
-    else capped(reinterpret_cast<float(&)[N]>(v), in, scale2, cap2, true);
+    for (int t = 0; t < N; t += 2) top = max3(top, fabsf(x[t]), fabsf(x[t + 1]));
+    if (!__all_sync(0xffffffffu, top * in <= 1.0f)) return false;
+    capped<NEAR, N>(x, in, scale2, cap2);
+    return true;
 }
 // Bias by distance from the head's table.  False (v then holds nothing) if an entry times log2 e
 // passes the lowest number.
@@ -345,6 +354,20 @@ __device__ __noinline__ void prepare_scores(const Args& a, uint32_t s_t, int d0,
         tmem_ld16(s_t + (uint32_t)c, v);
         tmem_ld_wait();
         score_piece(a, v, d0 + c, scale2, slope2, table);
+        tmem_st16(s_t + (uint32_t)c, v);
+    }
+    tmem_st_wait();
+}
+
+// Scores capped in TMEM 16 at a time, each by its own form.
+template <int KC>
+__device__ __noinline__ void prepare_capped(uint32_t s_t, float in, float scale2, float cap2) {
+#pragma unroll 1
+    for (int c = 0; c < KC; c += 16) {
+        uint32_t v[16];
+        tmem_ld16(s_t + (uint32_t)c, v);
+        tmem_ld_wait();
+        capped<EACH, 16>(reinterpret_cast<float*>(v), in, scale2, cap2);
         tmem_st16(s_t + (uint32_t)c, v);
     }
     tmem_st_wait();
@@ -906,7 +929,11 @@ __global__ void __launch_bounds__(NTHR, 2)
                     const int side = __all_sync(0xffffffffu, d0 >= 0) ? 1 : __all_sync(0xffffffffu, d0 + KC - 1 <= 0) ? -1 : 0;
                     scores_slopes(v, d0, side, scale2, slope2);
                 }
-                if constexpr (KIND == CAPPED) scores_capped(v, a.scale / a.cap, scale2, a.cap * LOG2E);
+                if constexpr (KIND == CAPPED)
+                    if (!scores_capped(v, a.scale / a.cap, scale2, a.cap * LOG2E)) {
+                        prepare_capped<KC>(s_t, a.scale / a.cap, scale2, a.cap * LOG2E);
+                        load();
+                    }
                 if constexpr (KIND == TABLE)
                     if (!scores_table(v, d0, a.radius, scale2, table)) {
                         prepare_scores<KC>(a, s_t, d0, scale2, slope2, table);

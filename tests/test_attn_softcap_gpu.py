@@ -11,7 +11,7 @@ from crispembed_b200 import binding
 pytestmark = pytest.mark.gpu
 
 BF, HF = torch.bfloat16, torch.float16
-CAPS = [3.0, 1e3, 1e4, 1e5, 1e6, 1e9, 1e30]
+CAPS = [3.0, 64.0, 65.0, 1e3, 1e4, 1e5, 1e6, 1e9, 1e30]
 
 
 def _attend(dev, dtype, rows, keys, heads, kv, hd, loud=None, **kw):
