@@ -2,7 +2,7 @@
 // rows times query heads.
 //
 // A 128-row tile would be empty but for those rows, and its chain of barriers sets the pace: 55 us
-// for the last tokens of 32 texts against up to 4096 keys, 16 heads of 128 on 4.  Here: 37 us, 4.1
+// for the last tokens of 32 texts against up to 4096 keys, 16 heads of 128 on 4.  Here: 38 us, 4.0
 // TB/s.  Every warp streams its own keys, 16 at a step, through a ring of its own in shared
 // memory (cp.async, no barrier between warps): m16n8k16 products with the rows as M, one
 // online softmax a warp, weights straight from the product's registers.  A product's 16 head
@@ -305,7 +305,7 @@ int launch_few(const Args& a, cudaStream_t st) {
     if (items > INT32_MAX / 8) return ceb_set_error(2, "attention_masked: %lld key heads", (long long)items);
     const int steps = (a.max_k + FKEYS - 1) / FKEYS;
     // Two blocks run on an SM; up to two waves of them are made, as long as a warp keeps four steps
-    // (32 texts: one wave 36.7 us, two 37.4, four 46.8, when the blocks' beginnings and ends show;
+    // (32 texts: one wave 37.5 us, two 37.8, four 47.6, when the blocks' beginnings and ends show;
     // a single text wants all it can get).
     int parts = 1;
     while (parts < 8 && items * parts * 2 <= 4 * ceb_num_sms() && steps >= 4 * FW * parts) parts *= 2;

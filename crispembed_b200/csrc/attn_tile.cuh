@@ -186,7 +186,7 @@ __device__ __noinline__ bool wait_over(volatile int* abort, int* err, uint32_t t
 // then still add up to one.  Adding them before the rounding leaves the output up to 1.4
 // (fp16) or 1.5 (bf16) times as far off as its own rounding when the maximum in use is not the row's last
 // one.  Here bf16 weights are added as rounded (3 % of the time, two bit operations a pair) and
-// fp16 ones are not (converting them back took 10 %).
+// fp16 ones are not (converting them back took 9 %).
 CEB_DEV f32x2 unpack(uint32_t u, __half) {
     const float2 f = __half22float2(u32_as_h2(u));
     return f2_pack(f.x, f.y);
@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(NTHR, 2)
             int t = SPLIT ? (int)((int64_t)total * part / parts) : 0;
             // A bias by distance is greatest near the row's place as a rule: its chunk comes first, so that
             // the maxima are found at once and O is not rescaled chunk by chunk on the way there (texts
-            // of 32 to 512 keys, slopes up to 0.1: 364 -> 356 us).
+            // of 32 to 512 keys, slopes up to 0.1: 357 -> 349 us; 4 x 4096: 447 -> 400 us).
             int turn = 0;
             if (!SPLIT && (a.slopes || a.table) && total > 0) {
                 const int near = max((it.i0 + last) / 2 + shift, 0) / KC;
@@ -1165,8 +1165,8 @@ int by_kind(const Args& a, cudaStream_t st) {
     if (a.slopes) return launch_tiles<T, HD, 64, SLOPES>(a, st);
     if (a.table) return launch_tiles<T, HD, 64, TABLE>(a, st);
     // 96 keys a chunk where there are many and nothing but their products to turn into weights: 4 x 4096
-    // rows, 12 heads of 64, 317 us (64 keys: 366 us).  Texts of 32 to 512 keys run out of them within a
-    // chunk or two: 271 us with 64 (96: 297 us).
+    // rows, 12 heads of 64, 314 us (64 keys: 376 us).  Texts of 32 to 512 keys run out of them within a
+    // chunk or two: 269 us with 64 (96: 304 us).
     if constexpr (HD == 64)
         if (a.max_k >= 1024) return launch_tiles<T, HD, 96, PLAIN>(a, st);
     return launch_tiles<T, HD, 64, PLAIN>(a, st);
